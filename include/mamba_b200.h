@@ -435,6 +435,83 @@ unsigned mb200_block_step_give_ups(void);
 int mb200_selftest_block_step_give_up(void* barriers, void* stream);
 int mb200_block_step(const mb200_block_step_args* args, float* scratch, void* barriers, void* stream);
 
+/* ---- Sequences of different lengths laid end to end (no reference counterpart; the reference pads a batch to one length).
+ * Sequence r is the rows cu_seqlens[r] .. cu_seqlens[r + 1] - 1 of (rows, channels) tensors; cu_seqlens has sequences + 1 entries that do
+ * not fall, the first of which counts as 0.  Rows from cu_seqlens[sequences] on belong to none: outputs are zero there.  All three arrays are on
+ * the device, read by the kernels alone, so that a captured graph can be replayed with other lengths; whatever they hold, nothing outside
+ * the tensors is touched.
+ * slots (sequences), or NULL: where in a pool of n_slots entries the sequence's state lies; one outside 0 .. n_slots - 1 means that it
+ * has none: it starts from zero and leaves nothing.  A slot that is given twice is left holding either sequence's state.  resume (sequences),
+ * or NULL for none: whether a sequence starts from what its slot holds.  A sequence without rows leaves its slot as it is. */
+typedef struct {
+  const int32_t* cu_seqlens;
+  int64_t sequences, rows;      /* at most 65534, and below 2^30 */
+  const int64_t* slots;
+  const uint8_t* resume;
+  int64_t n_slots;
+} mb200_packed;
+
+/* mb200_sscan_fwd over packed sequences.  x, delta, z, y: (rows, ED), Bm, Cm: (rows, N); states: the pool (n_slots, ED, N) float32, read
+ * and written in place, or NULL without slots.  carries (optional): mb200_packed_saved_states(rows, sequences) entries of ED x N floats for
+ * mb200_sscan_packed_bwd.  piece_len > 0 (a multiple of 16; d_state 16, tensors that tensor maps describe, otherwise MB200_EUNSUPPORTED) cuts
+ * sequences at every piece_len rows and scans the pieces side by side; pieces: 2 * mb200_packed_pieces(rows, sequences, piece_len) * ED * N floats. */
+int64_t mb200_packed_pieces(int64_t rows, int64_t sequences, int64_t piece_len);
+int64_t mb200_packed_saved_states(int64_t rows, int64_t sequences);
+int mb200_sscan_packed_fwd(const mb200_packed* seqs, const void* x, const void* delta, const void* z, const float* A, const void* Bm,
+                           const void* Cm, const float* D, const float* delta_bias, float* states, void* y, float* carries,
+                           float* pieces, int64_t ED, int N, int64_t x_sl, int64_t d_sl, int64_t z_sl, int64_t b_sl,
+                           int64_t c_sl, int64_t y_sl, int64_t piece_len, int dtype, int flags, void* stream);
+
+/* mb200_sscan_bwd over packed sequences without slots.  carries, pieces, piece_len: as the forward left them; piece_grads: scratch of
+ * mb200_packed_pieces(...) * ED * N floats.  dB, dC (rows, N), dA, dD, ddelta_bias: float32, ACCUMULATED into (caller zero-fills). */
+int mb200_sscan_packed_bwd(const mb200_packed* seqs, const void* x, const void* delta, const void* z, const float* A, const void* Bm,
+                           const void* Cm, const float* D, const float* delta_bias, const void* dy, const float* carries,
+                           const float* pieces, float* piece_grads, void* dx, void* ddelta, void* dz, float* dB, float* dC,
+                           float* dA, float* dD, float* ddelta_bias, int64_t ED, int N, int64_t x_sl, int64_t d_sl, int64_t z_sl,
+                           int64_t b_sl, int64_t c_sl, int64_t dy_sl, int64_t dx_sl, int64_t dd_sl, int64_t dz_sl,
+                           int64_t piece_len, int dtype, int flags, void* stream);
+
+/* mb200_conv1d_silu_fwd over packed sequences: taps before a sequence's first row are 0, or its slot's window if it resumes.  x, y: (rows, ED);
+ * windows: the pool (n_slots, ED, 3) in the activations' type, oldest input first, left holding each sequence's last three inputs, or NULL
+ * without slots. */
+int mb200_conv1d_silu_packed_fwd(const mb200_packed* seqs, const void* x, const float* w, const float* bias, void* windows, void* y,
+                                 int64_t ED, int K, int64_t x_sl, int64_t y_sl, int dtype, void* stream);
+/* Its backward, without slots; dw (ED, 4), dbias (ED, may be NULL): float32, ACCUMULATED into (caller zero-fills). */
+int mb200_conv1d_silu_packed_bwd(const mb200_packed* seqs, const void* x, const float* w, const float* bias, const void* dy,
+                                 void* dx, float* dw, float* dbias, int64_t ED, int K, int64_t x_sl, int64_t dy_sl,
+                                 int64_t dx_sl, int dtype, void* stream);
+
+/* mb200_ssm_step_params and mb200_conv_step on pools: row b's state is entry slots[b] of states (n_slots, ED, N), its window entry slots[b] of
+ * windows (n_slots, ED, K-1), both updated in place.  A row with a slot outside 0 .. n_slots - 1 gives zeros and updates nothing (padding of
+ * a captured batch).  A slot that is given twice is left holding either row's state. */
+int mb200_ssm_step_slots(const void* x, const void* delta, const void* z, const void* A, int A_dtype, int A_is_log,
+                         const void* Bm, const void* Cm, const void* D, int D_dtype, const void* delta_bias, int bias_dtype,
+                         float* states, const int64_t* slots, int64_t n_slots, void* y, int64_t B, int64_t ED, int N,
+                         int64_t x_sb, int64_t d_sb, int64_t z_sb, int64_t b_sb, int64_t c_sb, int64_t y_sb,
+                         int dtype, int flags, void* stream);
+int mb200_conv_step_slots(const void* xin, void* windows, const int64_t* slots, int64_t n_slots, const void* w, int w_dtype,
+                          const void* bias, int bias_dtype, void* xc, int64_t B, int64_t ED, int K, int64_t x_sb, int dtype, void* stream);
+
+/* ---- Beam search (no reference counterpart; the reference samples).
+ * Of the beams x V continuations of a group, value = scores[k] + logits[k,v] - logsumexp(logits[k]), the num highest, highest first, ties to the
+ * lowest k V + v.  logits: groups * beams rows of V, row_stride apart; scores (groups, beams).  finished (groups, beams), or NULL: a finished
+ * beam has one continuation, end_token, at its own score.  A beam whose score is not finite, or whose logits hold a NaN or +inf or nothing above
+ * -inf, has none.  Where a group has fewer than num, the rest are the lowest k V + v left, at -inf.
+ * Out: out_scores, out_tokens (v), out_parents (k), each (groups, num).  At most 64 beams, num at most 64 (MB200_ETOOBIG);
+ * scratch: mb200_beam_select_scratch_bytes bytes, 16-byte aligned, for one call at a time. */
+int64_t mb200_beam_select_scratch_bytes(int64_t groups, int64_t beams, int64_t V, int num);
+int mb200_beam_select(const void* logits, const float* scores, const uint8_t* finished, void* scratch, float* out_scores,
+                      int64_t* out_tokens, int64_t* out_parents, int64_t groups, int64_t beams, int64_t V, int num, int64_t end_token,
+                      int64_t row_stride, int dtype, void* stream);
+
+/* The slots of beams that go on from beams `parents` (groups, beams; numbers inside the group) of those that hold `slots` (groups, beams): the
+ * lowest child of a beam keeps its slot, the other children take the slots of beams without children, lowest first, and the entries of all
+ * n_pools pools are copied there in place: pools[i] holds n_slots entries of entry_bytes[i] bytes.  (pools and entry_bytes are on the HOST.)
+ * A parent outside 0 .. beams - 1 is nobody: its child takes a slot, and nothing is copied.  Slots outside 0 .. n_slots - 1 are handed on and
+ * nothing is copied to or from them.  Slots must differ.  At most 64 beams a group and 4096 in all (MB200_ETOOBIG). */
+int mb200_beam_reorder(const int64_t* slots, const int64_t* parents, int64_t* new_slots, int64_t groups, int64_t beams, int64_t n_slots,
+                       void* const* pools, const int64_t* entry_bytes, int n_pools, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,362 @@
+// Depthwise causal conv1d + SiLU (d_conv = 4) over sequences of different lengths laid end to end, forward and backward:
+//     y[t,e] = silu( bias[e] + sum_k w[e,k] * in(t-3+k, e) ),   in = x within the sequence of row t,
+// and before its first row 0 or, when the sequence resumes, the window that its slot holds.  Streaming, bound by HBM as the kernels on
+// rectangles are (conv1d.cu, whose mapping this follows: a thread owns V channels and walks a chunk of rows with the last three inputs
+// in registers, the loads of a group of rows in flight together).
+//
+// Where sequences begin is a bit per row, which a CTA gathers from cu_seqlens into shared memory for its own rows: one round of loads for up
+// to as many sequences as it has threads.  A group of rows in which none begins, which is nearly all of them, takes a path without tests.
+#include <type_traits>
+#include "conv1d.cuh"
+#include "packed.cuh"
+
+namespace mb200 {
+namespace {
+
+constexpr int kPkThreads = 256, kPkWarps = kPkThreads / 32;
+constexpr int kPkChunk = 32, kPkGroup = 8;
+constexpr int kPkRows = kPkWarps * kPkChunk;           // rows of a forward CTA
+
+// Of a pool of windows (n_slots, ED, 3): the windows of V neighbouring channels from e on, oldest input first.
+template <typename T, int V, int W>
+__device__ __forceinline__ void load_window(const T* p, Pk<W> (&win)[V / W][kConvK - 1]) {
+  float v[V * 3];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const CVec<T, V> q = cload<T, V>(p + k * V, true);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[k * V + i] = Elem<T>::to_f(q.v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < V / W; ++i)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      if constexpr (W == 1) win[i][k].v = v[3 * i + k];
+      else win[i][k].v = make_float2(v[6 * i + k], v[6 * i + 3 + k]);
+    }
+}
+
+// The thread that meets a sequence's first row also leaves the window: the only one that reads what the slot held.  So the (at most two) rows
+// after a first row that need it too, when they fall into the next chunk, are done by the chunk of the first row.
+template <typename T, int V>
+__global__ void __launch_bounds__(kPkThreads, 3)
+conv1d_silu_packed_fwd_kernel(const Packed seqs, const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ bias,
+                              T* __restrict__ y, T* windows, int64_t ED, int64_t x_sl, int64_t y_sl) {
+  constexpr int kBefore = kConvK - 2, kAfter = kConvK - 2;
+  __shared__ int s_first[kBefore + kPkRows + kAfter];     // 1 + the sequence whose first row this is, 0: none's
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int T0 = int(blockIdx.x) * kPkRows;
+  for (int i = threadIdx.x; i < kBefore + kPkRows + kAfter; i += kPkThreads) s_first[i] = 0;
+  __syncthreads();
+  const int tail = seqs.start(seqs.sequences);            // rows from here on belong to no sequence
+  for (int r = threadIdx.x; r < seqs.sequences; r += kPkThreads) {
+    const int first = seqs.start(r);
+    if (seqs.end(r, first) > first && first >= T0 - kBefore && first < T0 + kPkRows + kAfter) s_first[first - T0 + kBefore] = r + 1;
+  }
+  __syncthreads();
+  // bit i: a sequence begins at row t0 - 2 + i
+  constexpr int kSeen = kBefore + kPkChunk + kAfter;
+  static_assert(kSeen > 32 && kSeen <= 64, "two ballots");
+  const int* const mine = s_first + warp * kPkChunk;
+  const uint64_t firsts = uint64_t(__ballot_sync(0xffffffffu, mine[lane] != 0)) |
+                          uint64_t(__ballot_sync(0xffffffffu, lane < kSeen - 32 && mine[lane < kSeen - 32 ? 32 + lane : 0] != 0)) << 32;
+  const int64_t e = (int64_t(blockIdx.y) * 32 + lane) * V;
+  const int t0 = T0 + warp * kPkChunk;
+  if (e >= ED || t0 >= seqs.rows) return;
+  // rows this chunk does: from lo to hi
+  auto first_at = [&](int t) { return t - t0 + kBefore >= 0 && t - t0 + kBefore < kSeen && (firsts >> (t - t0 + kBefore) & 1); };
+  const int t1 = min(t0 + kPkChunk, seqs.rows);
+  int lo = t0, hi = min(t1, tail);
+  // a row within two of its sequence's first one, if that lies in another chunk, belongs to that chunk
+  constexpr int kFar = -2 * kConvK;
+  const int in_front = first_at(t0 - 1) ? t0 - 1 : first_at(t0 - 2) ? t0 - 2 : kFar;
+  const int at_end = t1 != t0 + kPkChunk ? kFar : first_at(t1 - 1) ? t1 - 1 : first_at(t1 - 2) ? t1 - 2 : kFar;
+  while (lo < t1 && lo - in_front < kConvK - 1 && !first_at(lo)) ++lo;
+  while (hi < tail && hi - at_end < kConvK - 1 && !first_at(hi)) ++hi;
+  constexpr int W = (V % 2 == 0) ? 2 : 1, P = V / W;
+  using F = Pk<W>;
+  F wk[P][kConvK], bv[P], win[P][kConvK - 1];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    bv[i] = bias ? F::load(bias + e + W * i, 1) : F::splat(0.f);
+#pragma unroll
+    for (int k = 0; k < kConvK; ++k) wk[i][k] = F::load(w + (e + W * i) * kConvK + k, kConvK);
+  }
+  const T* xp = x + int64_t(lo) * x_sl + e;
+  T* yp = y + int64_t(lo) * y_sl + e;
+#pragma unroll
+  for (int k = 0; k < kConvK - 1; ++k) {
+    F xv[P];
+    unpack<T, V, W>(cload<T, V>(xp + (k - (kConvK - 1)) * x_sl, lo + k >= kConvK - 1), xv);
+#pragma unroll
+    for (int i = 0; i < P; ++i) win[i][k] = xv[i];
+  }
+  // What row t, the first of sequence r, enters with; and what the sequence leaves.
+  auto begin = [&](int t, int r) {
+    const int64_t slot = windows ? seqs.slot(r) : -1;
+    T* const at = windows + (slot * ED + e) * (kConvK - 1);
+    const bool old = slot >= 0 && seqs.resumes(r);
+    if (old) load_window<T, V, W>(at, win);
+    else {
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+#pragma unroll
+        for (int k = 0; k < kConvK - 1; ++k) win[i][k] = F::splat(0.f);
+    }
+    if (slot < 0) return;
+    const int n = seqs.end(r, t) - t;
+    T v[kConvK - 1][V];
+#pragma unroll
+    for (int k = 0; k < kConvK - 1; ++k) {
+      const int place = n - (kConvK - 1) + k;             // of the input that goes to entry k
+      if (place >= 0) {
+        const CVec<T, V> q = cload<T, V>(x + int64_t(t + place) * x_sl + e, true);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[k][i] = q.v[i];
+      } else {                                            // shorter than the window: what was there moves up
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[k][i] = old ? at[3 * i + n + k] : Elem<T>::from_f(0.f);
+      }
+    }
+    CVec<T, V> out[kConvK - 1];
+#pragma unroll
+    for (int j = 0; j < (kConvK - 1) * V; ++j) out[j / V].v[j % V] = v[j % 3][j / 3];
+#pragma unroll
+    for (int k = 0; k < kConvK - 1; ++k) cstore<T, V>(at + k * V, out[k]);
+  };
+  auto group = [&](auto plain, int t) {                   // rows t .. t + 7 below hi; plain: all of them, and no sequence begins
+    constexpr bool kPlain = decltype(plain)::value;
+    CVec<T, V> v[kPkGroup];
+#pragma unroll
+    for (int j = 0; j < kPkGroup; ++j) {
+      v[j] = cload<T, V>(xp, kPlain || t + j < hi);
+      xp += x_sl;
+    }
+#pragma unroll
+    for (int j = 0; j < kPkGroup; ++j) {
+      if (!kPlain && t + j < hi && first_at(t + j)) begin(t + j, mine[t + j - t0 + kBefore] - 1);
+      F xn[P], o[P];
+      unpack<T, V, W>(v[j], xn);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        F acc = pfma(wk[i][0], win[i][0], bv[i]);
+        acc = pfma(wk[i][1], win[i][1], acc);
+        acc = pfma(wk[i][2], win[i][2], acc);
+        acc = pfma(wk[i][3], xn[i], acc);
+        win[i][0] = win[i][1]; win[i][1] = win[i][2]; win[i][2] = xn[i];
+        o[i] = pmul(acc, psigmoid(acc));
+      }
+      if (kPlain || t + j < hi) cstore<T, V>(yp, pack<T, V, W>(o));
+      yp += y_sl;
+    }
+  };
+  // No sequence begins in the chunk or in the two rows in front of it, and all of it is rows of sequences.
+  if (lo == t0 && hi == t0 + kPkChunk && (firsts & ((uint64_t(1) << (kBefore + kPkChunk)) - 1)) == 0) {
+#pragma unroll
+    for (int g = 0; g < kPkChunk / kPkGroup; ++g) group(std::true_type{}, t0 + g * kPkGroup);
+  } else {
+#pragma unroll 1
+    for (int t = lo; t < hi; t += kPkGroup) group(std::false_type{}, t);
+    CVec<T, V> zero;
+#pragma unroll
+    for (int i = 0; i < V; ++i) zero.v[i] = Elem<T>::from_f(0.f);
+    for (int t = max(t0, tail); t < t1; ++t) cstore<T, V>(y + int64_t(t) * y_sl + e, zero);
+  }
+}
+
+// dx[t] = sum_j w[3-j] * dpre[t+j] over the rows t+j of t's sequence;  dw[k] = sum_t dpre[t] * in(t-3+k);  dbias = sum dpre;
+// dpre[t] = dy[t] * silu'(pre[t]), pre recomputed from x.  Sequences that resume have no backward, so in = 0 before a first row.
+// As on rectangles the windows hold as many rows as a group, dx trails by three rows, and the 4 warps of a CTA add their sums in shared memory.
+constexpr int kPkBwdThreads = 128, kPkBwdWarps = kPkBwdThreads / 32, kPkBwdChunkMost = 64;
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kPkBwdThreads, 4)
+conv1d_silu_packed_bwd_kernel(const Packed seqs, const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ bias,
+                              const T* __restrict__ dy, T* __restrict__ dx, float* __restrict__ dw, float* __restrict__ dbias, int64_t ED,
+                              int64_t x_sl, int64_t dy_sl, int64_t dx_sl, int chunk) {
+  constexpr int kG = kConvK, kH = kConvK - 1;
+  constexpr int kBits = kH + kPkBwdWarps * kPkBwdChunkMost + kH;
+  __shared__ float s_acc[32 * V * (kConvK + 1)];          // per channel of the CTA: dw[0..3], dbias
+  __shared__ unsigned s_first[(kBits + 31) / 32 + 1];     // bit i: a sequence begins at row T0 - 3 + i
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int T0 = int(blockIdx.x) * kPkBwdWarps * chunk;
+  for (int i = threadIdx.x; i < 32 * V * (kConvK + 1); i += kPkBwdThreads) s_acc[i] = 0.f;
+  for (int i = threadIdx.x; i < (kBits + 31) / 32 + 1; i += kPkBwdThreads) s_first[i] = 0;
+  __syncthreads();
+  const int tail = seqs.start(seqs.sequences);
+  for (int r = threadIdx.x; r <= seqs.sequences; r += kPkBwdThreads) {
+    const int at = seqs.start(r) - (T0 - kH);
+    if (at >= 0 && at < kBits) atomicOr(&s_first[at >> 5], 1u << (at & 31));
+  }
+  __syncthreads();
+  const int64_t e = (int64_t(blockIdx.y) * 32 + lane) * V;
+  const int t0 = T0 + warp * chunk, t1 = min(seqs.rows, t0 + chunk);
+  if (e < ED && t0 < seqs.rows) {
+    constexpr int W = (V % 2 == 0) ? 2 : 1, P = V / W;
+    using F = Pk<W>;
+    F wk[P][kConvK], bv[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      bv[i] = bias ? F::load(bias + e + W * i, 1) : F::splat(0.f);
+#pragma unroll
+      for (int k = 0; k < kConvK; ++k) wk[i][k] = F::load(w + (e + W * i) * kConvK + k, kConvK);
+    }
+    F xw[P][kG], dw_[P][kG], dwacc[P][kConvK], dbacc[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      dbacc[i] = F::splat(0.f);
+#pragma unroll
+      for (int k = 0; k < kConvK; ++k) dwacc[i][k] = F::splat(0.f);
+#pragma unroll
+      for (int k = 0; k < kG; ++k) dw_[i][k] = F::splat(0.f);
+    }
+    // bits of rows t - 3 .. t + 3, lowest first
+    auto firsts_at = [&](int t) {
+      const int at = t - T0;
+      return __funnelshift_r(s_first[at >> 5], s_first[(at >> 5) + 1], at & 31) & 0x7fu;
+    };
+    const T* xg = x + int64_t(t0) * x_sl + e;
+    const T* gg = dy + int64_t(t0) * dy_sl + e;
+    T* og = dx + int64_t(t0 - kH) * dx_sl + e;
+    {
+      const unsigned f = firsts_at(t0) & 7u;              // of t0-3 .. t0-1: what lies before the last of them is not in the sequence
+#pragma unroll
+      for (int k = 0; k < kH; ++k) {
+        F xv[P];
+        unpack<T, V, W>(cload<T, V>(xg + (k - kH) * x_sl, t0 + k >= kH && t0 + k - kH < tail && (f >> (k + 1)) == 0), xv);
+#pragma unroll
+        for (int i = 0; i < P; ++i) xw[i][k + 1] = xv[i];
+      }
+    }
+    const F one = F::splat(1.f), mone = F::splat(-1.f), zero = F::splat(0.f);
+    const int own = t1 - t0, end = min(tail, t1 + kH) - t0;
+    auto group = [&](auto plain, int s0, unsigned f) {    // f: bits of rows s0 - 3 .. s0 + 3; plain: inside the chunk, and none set
+      constexpr bool kPlain = decltype(plain)::value;
+      CVec<T, V> qx[kG], qg[kG];
+#pragma unroll
+      for (int j = 0; j < kG; ++j) {
+        qx[j] = cload<T, V>(xg, kPlain || s0 + j < end);
+        qg[j] = cload<T, V>(gg, kPlain || s0 + j < end);
+        xg += x_sl; gg += dy_sl;
+      }
+#pragma unroll
+      for (int j = 0; j < kG; ++j) {
+        F g[P], xn[P], o[P];
+        unpack<T, V, W>(qg[j], g);
+        unpack<T, V, W>(qx[j], xn);
+        const bool fresh = !kPlain && (f >> (kH + j) & 1);
+        // how many rows behind t-3 its dx takes in: up to the first row of the next sequence
+        const int reach = kPlain ? 3 : f >> (j + 1) & 1 ? 0 : f >> (j + 2) & 1 ? 1 : f >> (j + 3) & 1 ? 2 : 3;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          if (fresh) {
+#pragma unroll
+            for (int k = 0; k < kG; ++k) xw[i][k] = zero;
+          }
+          xw[i][j] = xn[i];
+          F pre = bv[i];
+#pragma unroll
+          for (int k = 0; k < kConvK; ++k) pre = pfma(wk[i][k], xw[i][(j + 1 + k) % kG], pre);
+          const F sg = psigmoid(pre);
+          const F dp = pmul(pmul(g[i], sg), pfma(pre, pfma(sg, mone, one), one));
+          dw_[i][j] = dp;
+          // dx[t-3] = w3*dpre[t-3] + w2*dpre[t-2] + w1*dpre[t-1] + w0*dpre[t]
+          F acc = pmul(wk[i][kH], dw_[i][(j + 1) % kG]);
+#pragma unroll
+          for (int k = 1; k < kConvK; ++k)
+            if (kPlain || k <= reach) acc = pfma(wk[i][kH - k], dw_[i][(j + 1 + k) % kG], acc);
+          o[i] = acc;
+          if (kPlain || s0 + j < own) {
+            dbacc[i] = padd(dbacc[i], dp);
+#pragma unroll
+            for (int k = 0; k < kConvK; ++k) dwacc[i][k] = pfma(dp, xw[i][(j + 1 + k) % kG], dwacc[i][k]);
+          }
+        }
+        if (kPlain || (s0 + j >= kH && s0 + j - kH < own)) cstore<T, V>(og, pack<T, V, W>(o));
+        og += dx_sl;
+      }
+    };
+#pragma unroll 1
+    for (int s0 = 0; s0 < own + kH; s0 += kG) {
+      const unsigned f = firsts_at(t0 + s0);
+      if (f == 0 && s0 >= kH && s0 + kG <= own && s0 + kG <= end) group(std::true_type{}, s0, f);
+      else group(std::false_type{}, s0, f);
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+#pragma unroll
+      for (int u = 0; u < W; ++u) {
+        float* a = s_acc + (lane * V + i * W + u) * (kConvK + 1);
+#pragma unroll
+        for (int k = 0; k < kConvK; ++k) {
+          float val;
+          if constexpr (W == 1) val = dwacc[i][k].v; else val = u ? dwacc[i][k].v.y : dwacc[i][k].v.x;
+          atomicAdd(a + k, val);
+        }
+        float dbv;
+        if constexpr (W == 1) dbv = dbacc[i].v; else dbv = u ? dbacc[i].v.y : dbacc[i].v.x;
+        atomicAdd(a + kConvK, dbv);
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * V * (kConvK + 1); i += kPkBwdThreads) {
+    const int64_t ch = int64_t(blockIdx.y) * 32 * V + i / (kConvK + 1);
+    const int k = i % (kConvK + 1);
+    if (ch >= ED) continue;
+    if (k < kConvK) atomicAdd(dw + ch * kConvK + k, s_acc[i]);
+    else if (dbias) atomicAdd(dbias + ch, s_acc[i]);
+  }
+}
+
+int check_conv(const mb200_packed* seqs, int64_t ED, int K, int dtype) {
+  if (const int rc = packed_check(seqs)) return rc;
+  if (ED < 0) return MB200_EINVAL;
+  if (K != kConvK || ED > int64_t(65535) * 32) return MB200_ETOOBIG;
+  return dtype != MB200_F32 && dtype != MB200_BF16 ? MB200_EDTYPE : MB200_OK;
+}
+
+}  // namespace
+}  // namespace mb200
+
+using namespace mb200;
+
+extern "C" int mb200_conv1d_silu_packed_fwd(const mb200_packed* seqs, const void* x, const float* w, const float* bias, void* windows, void* y,
+                                            int64_t ED, int K, int64_t x_sl, int64_t y_sl, int dtype, void* stream) {
+  if (const int rc = check_conv(seqs, ED, K, dtype)) return rc;
+  if (seqs->rows == 0 || ED == 0) return MB200_OK;
+  if (!x || !w || !y || (seqs->slots && !windows)) return MB200_EINVAL;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int kv = 4;
+  const bool vec = conv_vec_ok(ED, kv, {x, y, (const void*)windows}, {x_sl, y_sl});
+  const int v = vec ? kv : 1;
+  const dim3 grid(unsigned((seqs->rows + kPkRows - 1) / kPkRows), unsigned((ED + 32 * int64_t(v) - 1) / (32 * int64_t(v))));
+  const Packed k = packed_of(*seqs, 0);
+  if (!seqs->slots) windows = nullptr;
+#define MB200_CONV_FWD(TT, VV) conv1d_silu_packed_fwd_kernel<TT, VV><<<grid, kPkThreads, 0, st>>>(k, (const TT*)x, w, bias, (TT*)y, (TT*)windows, ED, x_sl, y_sl)
+  if (dtype == MB200_F32) { if (vec) MB200_CONV_FWD(float, 4); else MB200_CONV_FWD(float, 1); }
+  else { if (vec) MB200_CONV_FWD(__nv_bfloat16, 4); else MB200_CONV_FWD(__nv_bfloat16, 1); }
+#undef MB200_CONV_FWD
+  return check_launch();
+}
+
+extern "C" int mb200_conv1d_silu_packed_bwd(const mb200_packed* seqs, const void* x, const float* w, const float* bias, const void* dy,
+                                            void* dx, float* dw, float* dbias, int64_t ED, int K, int64_t x_sl, int64_t dy_sl,
+                                            int64_t dx_sl, int dtype, void* stream) {
+  if (const int rc = check_conv(seqs, ED, K, dtype)) return rc;
+  if (seqs->rows == 0 || ED == 0) return MB200_OK;
+  if (!x || !w || !dy || !dx || !dw || seqs->slots) return MB200_EINVAL;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int kv = 4;
+  const bool vec = conv_vec_ok(ED, kv, {x, dy, (const void*)dx}, {x_sl, dy_sl, dx_sl});
+  const int v = vec ? kv : 1;
+  const int chunk = 32;
+  const dim3 grid(unsigned((seqs->rows + kPkBwdWarps * chunk - 1) / (kPkBwdWarps * chunk)), unsigned((ED + 32 * int64_t(v) - 1) / (32 * int64_t(v))));
+  const Packed k = packed_of(*seqs, 0);
+#define MB200_CONV_BWD(TT, VV) \
+  conv1d_silu_packed_bwd_kernel<TT, VV><<<grid, kPkBwdThreads, 0, st>>>(k, (const TT*)x, w, bias, (const TT*)dy, (TT*)dx, dw, dbias, ED, x_sl, dy_sl, dx_sl, chunk)
+  if (dtype == MB200_F32) { if (vec) MB200_CONV_BWD(float, 4); else MB200_CONV_BWD(float, 1); }
+  else { if (vec) MB200_CONV_BWD(__nv_bfloat16, 4); else MB200_CONV_BWD(__nv_bfloat16, 1); }
+#undef MB200_CONV_BWD
+  return check_launch();
+}

@@ -225,8 +225,24 @@ void product_into(const Tensor& out, const Tensor& a, const Tensor& b, float alp
 Tensor product(const Tensor& a, const Tensor& b);
 Tensor add_residual(const Tensor& x, const Tensor& residual);
 std::tuple<Tensor, Tensor> ssm_step(const Tensor& x, const OptTensor& h, const Tensor& delta, const Tensor& A, const Tensor& B,
-                                    const Tensor& C, const OptTensor& D, const OptTensor& z, const OptTensor& delta_bias, bool inplace);
-std::tuple<Tensor, Tensor> conv_step(const Tensor& x, const Tensor& inputs, const Tensor& weight, const OptTensor& bias, bool inplace);
+                                    const Tensor& C, const OptTensor& D, const OptTensor& z, const OptTensor& delta_bias, bool inplace,
+                                    const OptTensor& slots);
+std::tuple<Tensor, Tensor> conv_step(const Tensor& x, const Tensor& inputs, const Tensor& weight, const OptTensor& bias, bool inplace,
+                                     const OptTensor& slots);
+// packed sequences, pools of slots and beams (packed.cpp)
+void same_device(const Tensor& on, std::initializer_list<const Tensor*> ts);
+void check_pool(const Tensor& pool, at::IntArrayRef entry, at::ScalarType dt, const char* what);
+void written(const Tensor& pool);
+Tensor as_type(const Tensor& t, at::ScalarType dt, const char* what);
+Tensor selective_scan_packed(const Tensor& x, const Tensor& delta, const Tensor& A, const Tensor& B, const Tensor& C, const OptTensor& D,
+                             const OptTensor& z, const OptTensor& delta_bias, const Tensor& cu_seqlens, const OptTensor& states,
+                             const OptTensor& slots, const OptTensor& resume, std::optional<int64_t> max_length,
+                             std::optional<int64_t> piece_length);
+Tensor conv1d_silu_packed(const Tensor& x, const Tensor& weight, const OptTensor& bias, const Tensor& cu_seqlens, const OptTensor& windows,
+                          const OptTensor& slots, const OptTensor& resume);
+std::tuple<Tensor, Tensor, Tensor> beam_select(const Tensor& logits, const Tensor& scores, std::optional<int64_t> num, const OptTensor& finished,
+                                               std::optional<int64_t> end_token);
+Tensor beam_reorder(const Tensor& slots, const Tensor& parents, const std::vector<Tensor>& pools);
 
 Tensor block(const Tensor& x, const OptTensor& in_w, const OptTensor& out_w, const std::vector<OptTensor>& params, int64_t dt_rank,
              int64_t d_state, bool halve);
@@ -242,5 +258,6 @@ void selftest_queue_conversions(int64_t n);
 void selftest_block_step_give_up(const Tensor& on);
 
 int64_t pick_pieces(int64_t batch, int64_t length, int64_t width, bool grad);
+int64_t pick_piece_length(int64_t rows, int64_t sequences, int64_t longest, int64_t width, bool grad);
 
 }  // namespace mb200_host

@@ -19,6 +19,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("add_residual", &add_residual, NoGil());
   m.def("ssm_step", &ssm_step, NoGil());
   m.def("conv_step", &conv_step, NoGil());
+  m.def("selective_scan_packed", &selective_scan_packed, NoGil());
+  m.def("conv1d_silu_packed", &conv1d_silu_packed, NoGil());
+  m.def("beam_select", &beam_select, NoGil());
+  m.def("beam_reorder", &beam_reorder, NoGil());
   m.def("block", &block, NoGil());
   m.def("reversible", &reversible);
   m.def("block_step", &block_step, NoGil());

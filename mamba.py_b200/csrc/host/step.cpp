@@ -108,19 +108,69 @@ void selftest_block_step_give_up(const Tensor& on) {
   check(mb200_selftest_block_step_give_up(ptr(barrier_counters(on)), cuda_stream()), "mb200_selftest_block_step_give_up");
 }
 
+// On a pool: row b's state is entry slots[b], updated in place.
+static Tensor state_step_slots(const Tensor& x, const Tensor& states, const Tensor& delta, const Tensor& A_, const Tensor& B, const Tensor& C,
+                               const Tensor& D_, const Tensor& z, const Tensor& bias_, const Tensor& slots_) {
+  TORCH_CHECK(x.dim() == 2 && A_.dim() == 2 && states.defined(), "mamba_b200: a step on slots takes (B, channels) activations and a pool of states");
+  same_device(x, {&states, &delta, &A_, &B, &C, &D_, &z, &bias_, &slots_});
+  const auto dt = act_dtype(x, delta, z, B, C);
+  const int64_t n = x.size(0), W = x.size(1), N = A_.size(1);
+  shape_is(delta, {n, W}, "delta");
+  if (z.defined()) shape_is(z, {n, W}, "z");
+  shape_is(A_, {W, N}, "A");
+  shape_is(B, {n, N}, "B");
+  shape_is(C, {n, N}, "C");
+  numel_is(D_, W, "D");
+  numel_is(bias_, W, "delta_bias");
+  check_pool(states, {W, N}, at::kFloat, "states");
+  shape_is(slots_, {n}, "slots");
+  const Tensor xs = rows(x, dt), ds = rows(delta, dt), zs = rows(z, dt), Bs = rows(B, dt), Cs = rows(C, dt), slots = as_type(slots_, at::kLong, "slots");
+  Tensor A = small_param(A_);
+  if (reinterpret_cast<uintptr_t>(A.data_ptr()) % 16) A = A.clone(at::MemoryFormat::Contiguous);
+  const Tensor D = small_param(D_), bias = small_param(bias_), y = empty({n, W}, dt, xs);
+  check(mb200_ssm_step_slots(ptr(xs), ptr(ds), ptr(zs), ptr(A), code_of(A), false, ptr(Bs), ptr(Cs), ptr(D), code_of(D), ptr(bias), code_of(bias),
+                             fptr(states), static_cast<const int64_t*>(ptr(slots)), states.size(0), ptr(y), n, W, int(N), st(xs, 0), st(ds, 0),
+                             st(zs, 0), st(Bs, 0), st(Cs, 0), st(y, 0), dtype_code(dt), bias.defined() ? MB200_DELTA_SOFTPLUS : 0, cuda_stream()),
+        "mb200_ssm_step_slots");
+  written(states);
+  return y;
+}
+
+static Tensor window_step_slots(const Tensor& x, const Tensor& windows, const Tensor& weight, const Tensor& bias_, const Tensor& slots_) {
+  TORCH_CHECK(x.dim() == 2, "mamba_b200: a step on slots takes (B, channels) activations, got ", x.sizes());
+  same_device(x, {&windows, &weight, &bias_, &slots_});
+  const auto dt = act_dtype(x);
+  const int64_t n = x.size(0), W = x.size(1), K = weight.size(-1);
+  numel_is(weight, W * K, "the filter");
+  numel_is(bias_, W, "the bias");
+  check_pool(windows, {W, K - 1}, dt, "windows");
+  shape_is(slots_, {n}, "slots");
+  const Tensor xs = rows(x, dt), w = small_param(weight), bias = small_param(bias_), slots = as_type(slots_, at::kLong, "slots");
+  const Tensor xc = empty({n, W}, dt, xs);
+  check(mb200_conv_step_slots(ptr(xs), ptr(windows), static_cast<const int64_t*>(ptr(slots)), windows.size(0), ptr(w), code_of(w), ptr(bias),
+                              code_of(bias), ptr(xc), n, W, int(K), st(xs, 0), dtype_code(dt), cuda_stream()),
+        "mb200_conv_step_slots");
+  written(windows);
+  return xc;
+}
+
 std::tuple<Tensor, Tensor> ssm_step(const Tensor& x, const OptTensor& h, const Tensor& delta, const Tensor& A, const Tensor& B,
-                                    const Tensor& C, const OptTensor& D, const OptTensor& z, const OptTensor& bias, bool inplace) {
-  require_cuda(x, delta, A, B, C, value(D), value(z), value(bias), value(h));
+                                    const Tensor& C, const OptTensor& D, const OptTensor& z, const OptTensor& bias, bool inplace,
+                                    const OptTensor& slots) {
+  require_cuda(x, delta, A, B, C, value(D), value(z), value(bias), value(h), value(slots));
   const c10::cuda::CUDAGuard guard(x.device());
   const BelowAutograd guard_ad;
+  if (slots) return {state_step_slots(x, value(h), delta, A, B, C, value(D), value(z), value(bias), *slots), *h};
   const StateStep o = state_step(x, value(h), delta, A, false, B, C, value(D), value(z), value(bias), inplace);
   return {o.y, o.h};
 }
 
-std::tuple<Tensor, Tensor> conv_step(const Tensor& x, const Tensor& inputs, const Tensor& weight, const OptTensor& bias, bool inplace) {
-  require_cuda(x, inputs, weight, value(bias));
+std::tuple<Tensor, Tensor> conv_step(const Tensor& x, const Tensor& inputs, const Tensor& weight, const OptTensor& bias, bool inplace,
+                                     const OptTensor& slots) {
+  require_cuda(x, inputs, weight, value(bias), value(slots));
   const c10::cuda::CUDAGuard guard(x.device());
   const BelowAutograd guard_ad;
+  if (slots) return {window_step_slots(x, inputs, weight, value(bias), *slots), inputs};
   const WindowStep o = window_step(x, inputs, weight, value(bias), inplace);
   return {o.xc, o.window};
 }

@@ -1,7 +1,7 @@
 // Geometry and parameter blocks shared by the fused selective-scan kernels.
 #pragma once
 #include <initializer_list>
-#include "common.cuh"
+#include "packed.cuh"
 #include "tile.cuh"
 
 namespace mb200 {
@@ -118,6 +118,10 @@ struct SscanFwdParams {
   // side by side: h0, and the state and decay product of the passes without y, are then (B, pieces, ED, N).  A launch
   // covers launch_pieces of them from piece0.
   int64_t pieces = 1, piece_len = int64_t(1) << 40, piece0 = 0, launch_pieces = 1;
+  // Packed sequences (B = 1, L = rows; seqs.rows == 0: none).  h0 and hT are then the pool of states, and pieceP, pieceS (items, ED, N)
+  // what the carry pass leaves for the pieces of cut sequences.
+  Packed seqs;
+  float *pieceP = nullptr, *pieceS = nullptr;
 };
 
 struct SscanBwdParams {
@@ -130,6 +134,8 @@ struct SscanBwdParams {
   int64_t dx_sb, dx_sl, dd_sb, dd_sl, dz_sb, dz_sl;
   int flags;
   int64_t pieces = 1, piece_len = int64_t(1) << 40;      // as in the forward; g_in is then (B, pieces, ED, N)
+  Packed seqs;                                           // as in the forward; pieceG: what the reverse carry pass leaves
+  const float *pieceP = nullptr, *pieceG = nullptr;
 };
 
 }  // namespace mb200

@@ -87,7 +87,8 @@ __device__ __forceinline__ void red_add_v4(float* addr, float a, float b, float 
 // (Without a gate the sum for y, which only dz needs, is still formed and handed over: 501 us for 525 on 8 x 2048 x 1536 in bfloat16.)
 // Saved states that lie next to a channel's others instead of two by two are 8-byte loads 64 bytes apart: 556 us there for 525, 138 for 134
 // on 3 x 1003 x 1000.
-template <typename T, bool kRev, bool kSoftplus, bool kHasZ>
+// kPacked: the grid's second dimension numbers the pieces of packed sequences, as in the forward; a piece folds the carries of those behind it.
+template <typename T, bool kRev, bool kSoftplus, bool kHasZ, bool kPacked = false>
 __global__ void __launch_bounds__(kBwdThreads, 3)
 sscan_bwd_tma_kernel(const __grid_constant__ BwdMaps maps, const SscanBwdParams p) {
   using S = TmaBwdSmem<T>;
@@ -114,9 +115,21 @@ sscan_bwd_tma_kernel(const __grid_constant__ BwdMaps maps, const SscanBwdParams 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t e0 = int64_t(blockIdx.x) * kBTE;
   // times fit 32 bits on this path; what is 64-bit in the loops costs the recurrence warps spills
-  const int64_t b = blockIdx.y;
-  const int pc = int(blockIdx.z), t_lo = int(pc * p.piece_len), t_hi = int(min64(p.L, t_lo + p.piece_len));
+  const int64_t b = kPacked ? 0 : blockIdx.y;
+  PackedItem item{};
+  if constexpr (kPacked) item = packed_item<kBwdThreads>(p.seqs, int(blockIdx.y), tid);
+  const int pc = kPacked ? item.pc : int(blockIdx.z), t_lo = kPacked ? item.lo : int(pc * p.piece_len),
+            t_hi = kPacked ? item.hi : int(min64(p.L, t_lo + p.piece_len));
   const int cols_ok = int(min64(kBTE, p.ED - e0));
+  if constexpr (kPacked) {
+    if (item.seq == p.seqs.sequences) {                   // rows behind the last sequence
+      zero_rows<T, kBwdThreads>(static_cast<T*>(p.dx) + e0, p.dx_sl, t_lo, t_hi, cols_ok, tid);
+      zero_rows<T, kBwdThreads>(static_cast<T*>(p.ddelta) + e0, p.dd_sl, t_lo, t_hi, cols_ok, tid);
+      if (kHasZ) zero_rows<T, kBwdThreads>(static_cast<T*>(p.dz) + e0, p.dz_sl, t_lo, t_hi, cols_ok, tid);
+      return;
+    }
+    if (t_lo == t_hi) return;
+  }
   constexpr bool softplus = kSoftplus;
   constexpr bool has_z = kHasZ;
   const int ntiles = (t_hi - t_lo + kBTile - 1) / kBTile;
@@ -164,12 +177,27 @@ sscan_bwd_tma_kernel(const __grid_constant__ BwdMaps maps, const SscanBwdParams 
     float2 A2[2], gc[2], dAacc[2];                                    // [state]{channel}
     {
       const float* A0 = p.A + e * N + n0;
-      const float* g0 = p.g_in ? p.g_in + ((b * p.pieces + pc) * p.ED + e) * N + n0 : nullptr;
+      const float* g0 = !kPacked && p.g_in ? p.g_in + ((b * p.pieces + pc) * p.ED + e) * N + n0 : nullptr;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         A2[k] = make_float2(ok0 ? A0[k] * kLog2e : 0.f, ok1 ? A0[N + k] * kLog2e : 0.f);
         gc[k] = make_float2(ok0 && g0 ? g0[k] : 0.f, ok1 && g0 ? g0[N + k] : 0.f);
         dAacc[k] = make_float2(0.f, 0.f);
+      }
+      if constexpr (kPacked) {
+        const int last = item.first + item.pieces - 1;
+        for (int k = last; k > item.first + pc; --k) {
+          const int64_t at = (k * p.ED + e) * N + n0;
+          auto get = [&](const float* from, bool ok, int64_t more) { return ok ? *reinterpret_cast<const float2*>(from + at + more) : make_float2(0.f, 0.f); };
+          const float2 G0 = get(p.pieceG, ok0, 0), G1 = get(p.pieceG, ok1, N);
+          if (k == last) {                                // (nothing entered it, and its product was not formed)
+            gc[0] = make_float2(G0.x, G1.x); gc[1] = make_float2(G0.y, G1.y);
+          } else {
+            const float2 P0 = get(p.pieceP, ok0, 0), P1 = get(p.pieceP, ok1, N);
+            gc[0] = __ffma2_rn(make_float2(P0.x, P1.x), gc[0], make_float2(G0.x, G1.x));
+            gc[1] = __ffma2_rn(make_float2(P0.y, P1.y), gc[1], make_float2(G0.y, G1.y));
+          }
+        }
       }
     }
     // slot of this channel pair in the rows of the operand tile (even and odd rows are swizzled differently)
@@ -181,11 +209,11 @@ sscan_bwd_tma_kernel(const __grid_constant__ BwdMaps maps, const SscanBwdParams 
       return keep + __shfl_xor_sync(0xffffffffu, give, 1);
     };
     float4* const epo = s_ep + sp * 16 + (cp ^ ((sp & 1) * 4));
-    const int nchunks = int((p.L + kHalf - 1) / kHalf);
+    const int nchunks = kPacked ? (item.end - item.begin + kHalf - 1) / kHalf : int((p.L + kHalf - 1) / kHalf);
     // saved states of a chunk as [state]{channel}
     struct Pair { float2 v[2]; };
     const bool paired = (p.flags & MB200_PAIRED_STATES) != 0, wide = paired && ok1 && !(p.ED & 1);
-    const float* carry_base = p.carries + b * nchunks * p.ED * N + state_pair(paired, p.ED, N, e, sp);
+    const float* carry_base = p.carries + (kPacked ? item.begin / kHalf + item.seq : b * nchunks) * p.ED * N + state_pair(paired, p.ED, N, e, sp);
     auto load_carry = [&](int c) {
       Pair r;
       r.v[0] = r.v[1] = make_float2(0.f, 0.f);
@@ -202,7 +230,7 @@ sscan_bwd_tma_kernel(const __grid_constant__ BwdMaps maps, const SscanBwdParams 
       return r;
     };
     // Chunks are taken from the end of the scan to its start; the state entering the next one is fetched a chunk ahead.
-    const int c_lo = t_lo / kHalf, nch = 2 * ntiles;
+    const int c_lo = (kPacked ? t_lo - item.begin : t_lo) / kHalf, nch = 2 * ntiles;
     auto chunk_at = [&](int k) { return c_lo + (rev ? k : nch - 1 - k); };
     Pair carry_next = load_carry(chunk_at(0));
 
@@ -364,9 +392,13 @@ sscan_bwd_tma_kernel(const __grid_constant__ BwdMaps maps, const SscanBwdParams 
         for (int k = 0; k < 4; k += 2) {                   // two channels at a time (packed arithmetic)
           float2 dv = pair_f(&dv4.v[k]);
           sg[k / 2] = dq[k / 2] = make_float2(0.f, 0.f);
-          if (softplus) dv = softplus_sigmoid_fast2(__fadd2_rn(dv, make_float2(bias4[k], bias4[k + 1])), sg[k / 2]);
+          if (softplus) {
+            dv = __fadd2_rn(dv, make_float2(bias4[k], bias4[k + 1]));
+            dv = kPacked ? softplus_sigmoid_near2(dv, sg[k / 2]) : softplus_sigmoid_fast2(dv, sg[k / 2]);
+          }
           if (rr >= rows_ok) dv = make_float2(0.f, 0.f);
-          const float2 dx2 = __fmul2_rn(dv, pair_f(&xv.v[k]));
+          float2 dx2 = __fmul2_rn(dv, pair_f(&xv.v[k]));
+          if (kPacked && rr >= rows_ok) dx2 = make_float2(0.f, 0.f);          // x of the next sequence may be anything
           o[k] = dv;
           o[k + 1] = dx2;
           float2 g = pair_f(&yv4.v[k]);
@@ -378,6 +410,7 @@ sscan_bwd_tma_kernel(const __grid_constant__ BwdMaps maps, const SscanBwdParams 
             dq[k / 2] = __fmul2_rn(gs, __ffma2_rn(zf, __ffma2_rn(s, mone, one), one));
             g = __fmul2_rn(gs, zf);
           }
+          if (kPacked && rr >= rows_ok) g = make_float2(0.f, 0.f);
           dyo[k] = g.x;
           dyo[k + 1] = g.y;
         }
@@ -395,7 +428,8 @@ sscan_bwd_tma_kernel(const __grid_constant__ BwdMaps maps, const SscanBwdParams 
 #pragma unroll
       for (int i = 0; i < 2 * kBcVecs / 32; ++i) {
         const int v = lane + 32 * i, q = v % kBcVecs;                        // four states of one row of B, then of C
-        const Vec4<T> r4 = *reinterpret_cast<const Vec4<T>*>(rB + v * 4);
+        Vec4<T> r4 = *reinterpret_cast<const Vec4<T>*>(rB + v * 4);
+        if (kPacked && q * 4 / N >= rows_ok) r4 = Vec4<T>{};
         dst[4 * q + (v >= kBcVecs)] = make_float2(Elem<T>::to_f(r4.v[0]), Elem<T>::to_f(r4.v[1]));
         dst[4 * q + 2 + (v >= kBcVecs)] = make_float2(Elem<T>::to_f(r4.v[2]), Elem<T>::to_f(r4.v[3]));
       }
@@ -550,9 +584,14 @@ int bwd_tma_launch(const SscanBwdParams& p, cudaStream_t st) {
   MB200_BWD_PICK(true, false, false) MB200_BWD_PICK(true, false, true)
   MB200_BWD_PICK(true, true, false) MB200_BWD_PICK(true, true, true)
 #undef MB200_BWD_PICK
+  const bool packed = p.seqs.rows > 0;
+  if (packed) k = sp ? (hz ? sscan_bwd_tma_kernel<T, false, true, true, true> : sscan_bwd_tma_kernel<T, false, true, false, true>)
+                     : (hz ? sscan_bwd_tma_kernel<T, false, false, true, true> : sscan_bwd_tma_kernel<T, false, false, false, true>);
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess)
     return MB200_ELAUNCH;
-  dim3 grid(unsigned((p.ED + kBTE - 1) / kBTE), unsigned(p.B), unsigned(p.pieces));
+  const int64_t rows = packed ? packed_items(p.seqs.rows, p.seqs.sequences, p.seqs.piece) : p.B;
+  if (rows > 65535) return MB200_ETOOBIG;
+  dim3 grid(unsigned((p.ED + kBTE - 1) / kBTE), unsigned(rows), unsigned(p.pieces));
   k<<<grid, kBwdThreads, S::kBytes, st>>>(m, p);
   return check_launch();
 }
@@ -666,4 +705,55 @@ extern "C" int mb200_sscan_bwd(const void* x, const void* delta, const void* z, 
   return mb200_sscan_bwd_pieces(x, delta, z, A, Bm, Cm, D, delta_bias, dy, carries, g_in, dx, ddelta, dz, dB, dC, dA, dD, ddelta_bias, g_out,
                                 B, L, ED, N, x_sb, x_sl, d_sb, d_sl, z_sb, z_sl, b_sb, b_sl, c_sb, c_sl, dy_sb, dy_sl, dx_sb, dx_sl,
                                 dd_sb, dd_sl, dz_sb, dz_sl, dtype, flags, 1, 0, stream);
+}
+
+extern "C" int mb200_sscan_packed_bwd(const mb200_packed* seqs, const void* x, const void* delta, const void* z, const float* A, const void* Bm,
+                                      const void* Cm, const float* D, const float* delta_bias, const void* dy, const float* carries,
+                                      const float* pieces, float* piece_grads, void* dx, void* ddelta, void* dz, float* dB, float* dC,
+                                      float* dA, float* dD, float* ddelta_bias, int64_t ED, int N, int64_t x_sl, int64_t d_sl, int64_t z_sl,
+                                      int64_t b_sl, int64_t c_sl, int64_t dy_sl, int64_t dx_sl, int64_t dd_sl, int64_t dz_sl,
+                                      int64_t piece_len, int dtype, int flags, void* stream) {
+  if (const int rc = packed_check(seqs)) return rc;
+  if (ED < 0 || piece_len < 0 || piece_len % kBTile) return MB200_EINVAL;
+  if (dtype != MB200_F32 && dtype != MB200_BF16) return MB200_EDTYPE;
+  if (N != 8 && N != 16 && N != 32 && N != 64) return MB200_ENSTATE;
+  if (seqs->rows == 0 || ED == 0) return MB200_OK;
+  if (!x || !delta || !A || !Bm || !Cm || !dy || !carries || !dx || !ddelta || !dB || !dC || !dA || (z && !dz)) return MB200_EINVAL;
+  if ((flags & MB200_DELTA_SOFTPLUS) && !delta_bias) return MB200_EINVAL;
+  if (seqs->slots) return MB200_EINVAL;            // sequences that resume or leave a state have no gradient
+  if (flags & MB200_REVERSE) return MB200_EUNSUPPORTED;
+  if (!aligned16(carries) || !aligned16(pieces) || !aligned16(piece_grads)) return MB200_EALIGN;
+  if (piece_len && (!pieces || !piece_grads || N != 16)) return MB200_EINVAL;
+  SscanBwdParams p{};
+  p.x = x; p.delta = delta; p.z = z; p.Bm = Bm; p.Cm = Cm; p.dy = dy; p.A = A; p.D = D;
+  p.delta_bias = delta_bias; p.carries = carries;
+  p.dx = dx; p.ddelta = ddelta; p.dz = dz; p.dB = dB; p.dC = dC; p.dA = dA; p.dD = dD; p.ddelta_bias = ddelta_bias;
+  p.B = 1; p.L = seqs->rows; p.ED = ED;
+  p.x_sl = x_sl; p.d_sl = d_sl; p.z_sl = z_sl; p.b_sl = b_sl; p.c_sl = c_sl; p.dy_sl = dy_sl; p.dx_sl = dx_sl; p.dd_sl = dd_sl; p.dz_sl = dz_sl;
+  p.flags = flags & (MB200_DELTA_SOFTPLUS | MB200_GENERAL_DECAY | MB200_PAIRED_STATES);
+  p.seqs = packed_of(*seqs, piece_len);
+  p.pieceP = pieces; p.pieceG = piece_grads;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int es = dtype == MB200_F32 ? 4 : 2;
+  if (bwd_tma_path_ok(p, N, es)) {
+    int rc = MB200_OK;
+    if (piece_len) {                               // what leaves each piece to the left when nothing enters it from the right
+      SscanFwdParams c{};
+      c.x = dy; c.delta = delta; c.z = z; c.A = A; c.Bm = Cm; c.Cm = Cm; c.delta_bias = delta_bias;
+      c.B = 1; c.L = seqs->rows; c.ED = ED;
+      c.x_sl = dy_sl; c.d_sl = d_sl; c.z_sl = z_sl; c.b_sl = c.c_sl = c_sl;
+      c.flags = (p.flags & ~MB200_PAIRED_STATES) | MB200_REVERSE | kFlagCarryPass;
+      c.seqs = p.seqs;
+      c.pieceS = piece_grads;
+      rc = mb200_fwd_tma_try(c, N, dtype, st);
+    }
+    if (rc == MB200_OK) rc = dtype == MB200_F32 ? bwd_tma_launch<float>(p, st) : bwd_tma_launch<__nv_bfloat16>(p, st);
+    if (rc <= 0) return rc;
+  }
+  if (piece_len) return MB200_EUNSUPPORTED;
+  const int kv = dtype == MB200_F32 ? 4 : 8;
+  bool vec = ED % kv == 0;
+  for (const void* q : {x, delta, z, Bm, Cm, dy, (const void*)dx, (const void*)ddelta, (const void*)dz}) vec = vec && aligned16(q);
+  for (int64_t s : {x_sl, d_sl, b_sl, c_sl, dy_sl, dx_sl, dd_sl, z ? z_sl : 0, z ? dz_sl : 0}) vec = vec && s % kv == 0;
+  return dtype == MB200_F32 ? bwd_generic_launch_t<float>(p, N, vec, st) : bwd_generic_launch_t<__nv_bfloat16>(p, N, vec, st);
 }

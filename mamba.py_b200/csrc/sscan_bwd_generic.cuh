@@ -45,7 +45,7 @@ template <typename T, int N> struct GenBwdSmem {
   static constexpr int kBytes = kFloats * 4;
 };
 
-template <typename T, int N, int KV>
+template <typename T, int N, int KV, bool kPacked = false>
 __global__ void __launch_bounds__(kThreadsPerCta)
 sscan_bwd_generic_kernel(const SscanBwdParams p) {
   using G = SscanGeom<N>;
@@ -70,21 +70,32 @@ sscan_bwd_generic_kernel(const SscanBwdParams p) {
   float* s_eC = s_eB + S::kEredStride;
   const int64_t e0 = int64_t(blockIdx.x) * kTE;
   const int64_t e = e0 + e_l;
-  const int64_t b = blockIdx.y;
+  const int64_t b = kPacked ? 0 : blockIdx.y;
+  PackedItem item{};
+  if constexpr (kPacked) item = packed_item<kThreadsPerCta>(p.seqs, int(blockIdx.y), threadIdx.x);
+  const int64_t row0 = kPacked ? item.lo : 0, L = kPacked ? item.hi - item.lo : p.L;
   const bool e_ok = e < p.ED;
   const int cols_ok = int(min64(kTE, p.ED - e0));
   const bool has_z = p.z != nullptr;
   const bool softplus = (p.flags & MB200_DELTA_SOFTPLUS) != 0;
 
-  const T* gx = static_cast<const T*>(p.x) + b * p.x_sb + e0;
-  const T* gd = static_cast<const T*>(p.delta) + b * p.d_sb + e0;
-  const T* gz = has_z ? static_cast<const T*>(p.z) + b * p.z_sb + e0 : nullptr;
-  const T* gdy = static_cast<const T*>(p.dy) + b * p.dy_sb + e0;
-  const T* gB = static_cast<const T*>(p.Bm) + b * p.b_sb;
-  const T* gC = static_cast<const T*>(p.Cm) + b * p.c_sb;
-  T* odx = static_cast<T*>(p.dx) + b * p.dx_sb + e0;
-  T* odd = static_cast<T*>(p.ddelta) + b * p.dd_sb + e0;
-  T* odz = has_z ? static_cast<T*>(p.dz) + b * p.dz_sb + e0 : nullptr;
+  if constexpr (kPacked) {
+    if (item.seq == p.seqs.sequences) {
+      zero_rows<T, kThreadsPerCta>(static_cast<T*>(p.dx) + e0, p.dx_sl, item.lo, item.hi, cols_ok, tid);
+      zero_rows<T, kThreadsPerCta>(static_cast<T*>(p.ddelta) + e0, p.dd_sl, item.lo, item.hi, cols_ok, tid);
+      if (has_z) zero_rows<T, kThreadsPerCta>(static_cast<T*>(p.dz) + e0, p.dz_sl, item.lo, item.hi, cols_ok, tid);
+    }
+    if (item.seq == p.seqs.sequences || L == 0) return;
+  }
+  const T* gx = static_cast<const T*>(p.x) + b * p.x_sb + row0 * p.x_sl + e0;
+  const T* gd = static_cast<const T*>(p.delta) + b * p.d_sb + row0 * p.d_sl + e0;
+  const T* gz = has_z ? static_cast<const T*>(p.z) + b * p.z_sb + row0 * p.z_sl + e0 : nullptr;
+  const T* gdy = static_cast<const T*>(p.dy) + b * p.dy_sb + row0 * p.dy_sl + e0;
+  const T* gB = static_cast<const T*>(p.Bm) + b * p.b_sb + row0 * p.b_sl;
+  const T* gC = static_cast<const T*>(p.Cm) + b * p.c_sb + row0 * p.c_sl;
+  T* odx = static_cast<T*>(p.dx) + b * p.dx_sb + row0 * p.dx_sl + e0;
+  T* odd = static_cast<T*>(p.ddelta) + b * p.dd_sb + row0 * p.dd_sl + e0;
+  T* odz = has_z ? static_cast<T*>(p.dz) + b * p.dz_sb + row0 * p.dz_sl + e0 : nullptr;
 
   float A2[4], gc[4], dAacc[4];
 #pragma unroll
@@ -98,10 +109,10 @@ sscan_bwd_generic_kernel(const SscanBwdParams p) {
 
   ActRegs rx, rd, rz, rdy;
   BcRegs rB, rC;
-  const int64_t nchunks = (p.L + kChunk - 1) / kChunk;
+  const int64_t nchunks = (L + kChunk - 1) / kChunk, chunk0 = kPacked ? item.begin / kChunk + item.seq : b * nchunks;
 
   auto fetch = [&](int64_t t0) {
-    const int rows_ok = int(min64(kChunk, p.L - t0));
+    const int rows_ok = int(min64(kChunk, L - t0));
     rx.load(gx + t0 * p.x_sl, p.x_sl, rows_ok, cols_ok, tid);
     rd.load(gd + t0 * p.d_sl, p.d_sl, rows_ok, cols_ok, tid);
     rdy.load(gdy + t0 * p.dy_sl, p.dy_sl, rows_ok, cols_ok, tid);
@@ -110,7 +121,7 @@ sscan_bwd_generic_kernel(const SscanBwdParams p) {
     rC.load(gC + t0 * p.c_sl, p.c_sl, rows_ok, N, tid);
   };
   auto commit = [&](int buf, int64_t t0) {
-    const int rows_ok = int(min64(kChunk, p.L - t0));
+    const int rows_ok = int(min64(kChunk, L - t0));
 #pragma unroll
     for (int i = 0; i < ActRegs::Map::kPerThread; ++i) {
       if (!ActRegs::Map::owns(i, tid)) continue;
@@ -146,7 +157,7 @@ sscan_bwd_generic_kernel(const SscanBwdParams p) {
   };
   auto load_carry = [&](int64_t c, float (&hp)[4]) {
     if (e_ok) {
-      const float4 v = load_states(p.carries + (b * nchunks + c) * p.ED * N, (p.flags & MB200_PAIRED_STATES) != 0, p.ED, N, e, q);
+      const float4 v = load_states(p.carries + (chunk0 + c) * p.ED * N, (p.flags & MB200_PAIRED_STATES) != 0, p.ED, N, e, q);
       hp[0] = v.x; hp[1] = v.y; hp[2] = v.z; hp[3] = v.w;
     } else {
       hp[0] = hp[1] = hp[2] = hp[3] = 0.f;
@@ -264,7 +275,7 @@ sscan_bwd_generic_kernel(const SscanBwdParams p) {
 
     // ---- write the chunk's dx, ddelta, dz tiles and flush its dB, dC block
     {
-      const int rows_ok = int(min64(kChunk, p.L - t0));
+      const int rows_ok = int(min64(kChunk, L - t0));
 #pragma unroll
       for (int i = 0; i < ActRegs::Map::kPerThread; ++i) {
         if (!ActRegs::Map::owns(i, tid)) continue;
@@ -286,7 +297,7 @@ sscan_bwd_generic_kernel(const SscanBwdParams p) {
         const float v = s_acc[i];
         s_acc[i] = 0.f;
         if (rr < rows_ok)
-          atomicAdd((which ? p.dC : p.dB) + (b * p.L + t0 + rr) * N + n, v);
+          atomicAdd((which ? p.dC : p.dB) + (b * p.L + row0 + t0 + rr) * N + n, v);
       }
     }
     if (c > 0) commit(buf ^ 1, t0 - kChunk);
@@ -318,11 +329,11 @@ template <typename T, int N>
 int bwd_generic_launch_n(const SscanBwdParams& p, bool vec, cudaStream_t st) {
   using G = SscanGeom<N>;
   using S = GenBwdSmem<T, N>;
-  dim3 grid(unsigned((p.ED + G::kTE - 1) / G::kTE), unsigned(p.B));
+  const bool packed = p.seqs.rows > 0;
+  dim3 grid(unsigned((p.ED + G::kTE - 1) / G::kTE), unsigned(packed ? p.seqs.sequences + 1 : p.B));
   constexpr int KV = Elem<T>::kVec;
-  auto kv = sscan_bwd_generic_kernel<T, N, KV>;
-  auto k1 = sscan_bwd_generic_kernel<T, N, 1>;
-  auto k = vec ? kv : k1;
+  auto k = packed ? (vec ? sscan_bwd_generic_kernel<T, N, KV, true> : sscan_bwd_generic_kernel<T, N, 1, true>)
+                  : (vec ? sscan_bwd_generic_kernel<T, N, KV> : sscan_bwd_generic_kernel<T, N, 1>);
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess)
     return MB200_ELAUNCH;
   k<<<grid, kThreadsPerCta, S::kBytes, st>>>(p);

@@ -158,7 +158,12 @@ __device__ __forceinline__ bool s4d_structured(const float* a4, float a0, int q)
 // p.carries (a template parameter because the test alone costs the recurrence warps 3 % of a prompt and 4 to 14 % of a carry pass:
 // 78.3 -> 80.9 us for 2048 steps of one CTA per SM, 52.7 -> 59.9 for 23 of 24 pieces of 53013 x 64).  Without y and kSave it is a carry pass,
 // which returns every piece's state; without y but with kSave a scan, which returns a row's last and saves states if there is p.carries.
-template <typename T, int N, bool kRev, bool kCarry, bool kHasY, bool kSave, bool kWide = false>
+// kPacked: the grid's second dimension numbers the pieces of the packed sequences `p.seqs`.  A box that reaches past a piece's last row
+// then holds rows of the next sequence, whose values the converter drops (0 * NaN would not).  The first piece of a cut sequence enters from
+// the slot in the carry pass already, which keeps what the slot held for the first piece of the scan (the last one may have written
+// the slot by then) in the place of the last piece's carry, which nobody needs.  The scan folds the carries of the pieces in front
+// of its own as it starts: a few loads in flight together, where a launch of their own takes 4 us.
+template <typename T, int N, bool kRev, bool kCarry, bool kHasY, bool kSave, bool kWide = false, bool kPacked = false>
 __global__ void __launch_bounds__(FwdGeom<N, kWide>::kThreads, FwdGeom<N, kWide>::kOcc)
 sscan_fwd_tma_kernel(const __grid_constant__ FwdMaps maps, const SscanFwdParams p) {
   using G = FwdGeom<N, kWide>;
@@ -181,14 +186,26 @@ sscan_fwd_tma_kernel(const __grid_constant__ FwdMaps maps, const SscanFwdParams 
 
   const int tid = threadIdx.x;
   const int64_t e0 = int64_t(blockIdx.x) * kTE;
-  const int64_t b = blockIdx.y;
-  const int pc = int(blockIdx.z + p.piece0), t_lo = int(pc * p.piece_len), t_hi = int(min64(p.L, t_lo + p.piece_len));
-  const int64_t slot = b * p.pieces + pc;
+  const int64_t b = kPacked ? 0 : blockIdx.y;
+  PackedItem item{};
+  if constexpr (kPacked) item = packed_item<G::kThreads>(p.seqs, int(blockIdx.y), tid);
+  const int pc = kPacked ? item.pc : int(blockIdx.z + p.piece0), t_lo = kPacked ? item.lo : int(pc * p.piece_len),
+            t_hi = kPacked ? item.hi : int(min64(p.L, t_lo + p.piece_len));
+  const int64_t slot = kPacked ? int64_t(item.first + pc) : b * p.pieces + pc;
   const int cols_ok = int(min64(kTE, p.ED - e0));
   const bool softplus = (p.flags & MB200_DELTA_SOFTPLUS) != 0;
   constexpr bool has_y = kHasY, kEvery = !kHasY && !kSave;
   const bool has_z = p.z != nullptr;
   const int ntiles = (t_hi - t_lo + kTile - 1) / kTile;
+  int64_t pool = -1;                                      // this sequence's slot
+  if constexpr (kPacked) {
+    if (item.seq == p.seqs.sequences) {                   // rows behind the last sequence
+      if (has_y) zero_rows<T, G::kThreads>(static_cast<T*>(p.y) + e0, p.y_sl, t_lo, t_hi, cols_ok, tid);
+      return;
+    }
+    if (ntiles == 0 || (kEvery && pc == (kCarry ? 0 : item.pieces - 1))) return;       // no rows; nothing follows (precedes) the last (first) piece
+    pool = p.seqs.slot(item.seq);
+  }
   // Direction.  With MB200_REVERSE time is walked from L-1 down to 0: processing tile kt is the
   // tile of timesteps starting at tile_t0(kt), and processing step s of a tile is its row 15 - s.
   // Saved states are indexed by TIME chunk either way: entry c is the state entering chunk c in the
@@ -230,7 +247,29 @@ sscan_fwd_tma_kernel(const __grid_constant__ FwdMaps maps, const SscanFwdParams 
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         a4[j] = e_ok[i] ? p.A[e * N + 4 * q + j] * kLog2e : 0.f;
-        h4[j] = (e_ok[i] && p.h0) ? p.h0[(slot * p.ED + e) * N + 4 * q + j] : 0.f;
+        h4[j] = (!kPacked && e_ok[i] && p.h0) ? p.h0[(slot * p.ED + e) * N + 4 * q + j] : 0.f;
+      }
+      if constexpr (kPacked && !kCarry) {
+        if (e_ok[i]) {
+          const int64_t at = e * N + 4 * q, each = p.ED * N;
+          auto put = [&](float4 v) { h4[0] = v.x; h4[1] = v.y; h4[2] = v.z; h4[3] = v.w; };
+          auto get = [&](const float* from, int64_t k) { return *reinterpret_cast<const float4*>(from + k * each + at); };
+          if (pc == 0) {
+            if (pool >= 0 && p.seqs.resumes(item.seq)) {
+              const int64_t kept = item.first + item.pieces - 1;
+              const bool cut = item.pieces > 1;
+              put(!kEvery && cut ? get(p.pieceS, kept) : get(p.h0, pool));
+              if (kEvery && cut) *reinterpret_cast<float4*>(p.pieceS + kept * each + at) = make_float4(h4[0], h4[1], h4[2], h4[3]);
+            }
+          } else if constexpr (!kEvery) {
+            put(get(p.pieceS, item.first));
+#pragma unroll 4
+            for (int k = item.first + 1; k < item.first + pc; ++k) {
+              const float4 P = get(p.pieceP, k), S = get(p.pieceS, k);
+              put(make_float4(fmaf(P.x, h4[0], S.x), fmaf(P.y, h4[1], S.y), fmaf(P.z, h4[2], S.z), fmaf(P.w, h4[3], S.w)));
+            }
+          }
+        }
       }
       A0[i] = e_ok[i] ? p.A[e * N] * kLog2e : 0.f;
       structured = structured && s4d_structured(a4, A0[i], q);
@@ -246,11 +285,12 @@ sscan_fwd_tma_kernel(const __grid_constant__ FwdMaps maps, const SscanFwdParams 
     } else {
       yp_off0 = yp_off1 = ((e_l >> 2) * 4 + q) * 4 + (e_l & 3);   // [channel quad][q][channel in quad]
     }
-    const int64_t nchunks = (p.L + kChunk - 1) / kChunk;
+    const int64_t chunk0 = kPacked ? item.begin / kChunk + item.seq + (t_lo - item.begin) / kChunk
+                                   : b * ((p.L + kChunk - 1) / kChunk) + tile_t0(0) / kChunk + (rev ? 1 : 0);
     const bool paired = (p.flags & MB200_PAIRED_STATES) != 0;
     // where the state entering the next chunk goes: one entry on (back, in reverse) per chunk
     const int64_t e_first = e0 + e_l;
-    float* carry_ptr = p.carries + (b * nchunks + tile_t0(0) / kChunk + (rev ? 1 : 0)) * p.ED * N +
+    float* carry_ptr = p.carries + chunk0 * p.ED * N +
                        (paired ? state_pair(true, p.ED, N, e_first, 2 * q) : e_first * N + 4 * q);
     const int64_t carry_step = rev ? -p.ED * N : p.ED * N;
     const int carry_i = paired ? 2 : N;                                      // from a channel to the next
@@ -321,7 +361,7 @@ sscan_fwd_tma_kernel(const __grid_constant__ FwdMaps maps, const SscanFwdParams 
 #pragma unroll
         for (int t = 0; t < kTile; ++t) {
           if (kSave && t % kChunk == 0 && (kHasY || p.carries)) {            // state entering this chunk
-            if (t0a + (rev ? kChunk - t : t) < p.L) {
+            if (t0a + (rev ? kChunk - t : t) < (kPacked ? t_hi : p.L)) {
 #pragma unroll
               for (int i = 0; i < kCPT; ++i) {
                 float* dst = carry_ptr + i * carry_i;
@@ -396,7 +436,11 @@ sscan_fwd_tma_kernel(const __grid_constant__ FwdMaps maps, const SscanFwdParams 
     const bool ok = structured ? run_tiles(std::true_type{}) : run_tiles(std::false_type{});
     if (!ok) return;
     // the scan itself returns the state that leaves its last piece, the carry passes every piece's
-    if (p.hT && (kEvery || pc == (rev ? 0 : p.pieces - 1))) {
+    if constexpr (kPacked) {
+      float* to = kEvery ? p.pieceS + slot * p.ED * N : pool >= 0 && pc == item.pieces - 1 ? p.hT + pool * p.ED * N : nullptr;
+      if (to && e_ok[0])
+        *reinterpret_cast<float4*>(to + (e0 + e_l) * N + 4 * q) = make_float4(hlo[0].x, hlo[0].y, hhi[0].x, hhi[0].y);
+    } else if (p.hT && (kEvery || pc == (rev ? 0 : p.pieces - 1))) {
 #pragma unroll
       for (int i = 0; i < kCPT; ++i)
         if (e_ok[i])
@@ -404,11 +448,12 @@ sscan_fwd_tma_kernel(const __grid_constant__ FwdMaps maps, const SscanFwdParams 
               make_float4(hlo[i].x, hlo[i].y, hhi[i].x, hhi[i].y);
     }
     if constexpr (kWantP) {
-      if (p.pT) {
+      float* const pT = kPacked ? p.pieceP : p.pT;
+      if (pT) {
 #pragma unroll
         for (int i = 0; i < kCPT; ++i)
           if (e_ok[i])
-            *reinterpret_cast<float4*>(p.pT + (slot * p.ED + e0 + e_l + i) * N + 4 * q) =
+            *reinterpret_cast<float4*>(pT + (slot * p.ED + e0 + e_l + i) * N + 4 * q) =
                 make_float4(ex2f(A2lo[i].x * dsum[i]), ex2f(A2lo[i].y * dsum[i]), ex2f(A2hi[i].x * dsum[i]),
                             ex2f(A2hi[i].y * dsum[i]));
       }
@@ -481,13 +526,18 @@ sscan_fwd_tma_kernel(const __grid_constant__ FwdMaps maps, const SscanFwdParams 
 #pragma unroll
         for (int k = 0; k < 4; k += 2) {
           float2 dv = pair_f(&dv4.v[k]);
-          if (softplus) dv = softplus_fast2(__fadd2_rn(dv, make_float2(bias4[k], bias4[k + 1])));
+          if (softplus) {
+            dv = __fadd2_rn(dv, make_float2(bias4[k], bias4[k + 1]));
+            dv = kPacked ? softplus_near2(dv) : softplus_fast2(dv);
+          }
           if (rr >= rows_ok) dv = make_float2(0.f, 0.f);    // past the end of the sequence
           float2 g = pair_f(&xv.v[k]);                      // x, or dy in its place
+          if (kPacked && rr >= rows_ok) g = make_float2(0.f, 0.f);
           if constexpr (kCarry) {
             if (has_z) {
               const float2 zf = pair_f(&zv4.v[k]);
               g = __fmul2_rn(g, __fmul2_rn(zf, sigmoid_fast2(zf)));
+              if (kPacked && rr >= rows_ok) g = make_float2(0.f, 0.f);
             }
           } else {
             g = __fmul2_rn(dv, g);
@@ -506,7 +556,8 @@ sscan_fwd_tma_kernel(const __grid_constant__ FwdMaps maps, const SscanFwdParams 
       for (int it = 0; it < (2 * kBcVecs + kNP - 1) / kNP; ++it) {
         const int v = pt + it * kNP;
         if (2 * kBcVecs % kNP && v >= 2 * kBcVecs) break;
-        const Vec4<T> r4 = *reinterpret_cast<const Vec4<T>*>(rB + v * 4);
+        Vec4<T> r4 = *reinterpret_cast<const Vec4<T>*>(rB + v * 4);
+        if (kPacked && v % kBcVecs * 4 / N >= rows_ok) r4 = Vec4<T>{};
         float* dst = (v < kBcVecs) ? dstB + v * 4 : dstC + (v - kBcVecs) * 4;
         *reinterpret_cast<float4*>(dst) = make_float4(Elem<T>::to_f(r4.v[0]), Elem<T>::to_f(r4.v[1]),
                                                       Elem<T>::to_f(r4.v[2]), Elem<T>::to_f(r4.v[3]));
@@ -596,6 +647,24 @@ sscan_fwd_tma_kernel(const __grid_constant__ FwdMaps maps, const SscanFwdParams 
   }
 }
 
+// The packed forms: the scan, with and without saved states, and (d_state 16, where sequences are cut) the two carry passes.
+template <typename T, int N, bool kWide>
+int tma_launch_packed(const FwdMaps& m, const SscanFwdParams& p, bool every, cudaStream_t st) {
+  using G = FwdGeom<N, kWide>;
+  using S = TmaFwdSmem<T, N, kWide>;
+  void (*k)(const FwdMaps, const SscanFwdParams) =
+      p.carries ? sscan_fwd_tma_kernel<T, N, false, false, true, true, kWide, true> : sscan_fwd_tma_kernel<T, N, false, false, true, false, kWide, true>;
+  if constexpr (N == 16 && !kWide) {
+    if (every) k = p.flags & kFlagCarryPass ? sscan_fwd_tma_kernel<T, N, true, true, false, false, false, true>
+                                            : sscan_fwd_tma_kernel<T, N, false, false, false, false, false, true>;
+  }
+  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess) return MB200_ELAUNCH;
+  const int64_t items = packed_items(p.seqs.rows, p.seqs.sequences, p.seqs.piece);
+  if (items > 65535) return MB200_ETOOBIG;
+  k<<<dim3(unsigned((p.ED + G::kTE - 1) / G::kTE), unsigned(items)), G::kThreads, S::kBytes, st>>>(m, p);
+  return check_launch();
+}
+
 template <typename T, int N, bool kWide>
 int tma_launch_tile(const SscanFwdParams& p, cudaStream_t st) {
   using G = FwdGeom<N, kWide>;
@@ -609,6 +678,7 @@ int tma_launch_tile(const SscanFwdParams& p, cudaStream_t st) {
   if (ok && p.z) ok = tma_encode(&m.z, p.z, bf, p.B, p.L, p.ED, p.z_sb, p.z_sl, G::kTE, kTile);
   else if (ok) m.z = m.x;
   if (!ok) return 1;                                   // caller falls back to the generic path
+  if (p.seqs.rows) return tma_launch_packed<T, N, kWide>(m, p, !p.y, st);
   const bool rv = (p.flags & MB200_REVERSE) != 0, hy = p.y != nullptr;
   const bool sv = p.carries != nullptr || (!hy && !p.pT && p.pieces > 1);
   void (*k)(const FwdMaps, const SscanFwdParams) = nullptr;
@@ -630,7 +700,7 @@ template <typename T, int N>
 int tma_launch_n(const SscanFwdParams& p, cudaStream_t st) {
   if constexpr (N == 16) {
     if (p.y && !(p.flags & kFlagCarryPass)) {
-      const int64_t sms = sm_count(), rows = p.B * p.launch_pieces, narrow = FwdGeom<N>::kTE, wide = FwdGeom<N, true>::kTE;
+      const int64_t sms = sm_count(), rows = p.seqs.rows ? packed_items(p.seqs.rows, p.seqs.sequences, p.seqs.piece) - 1 : p.B * p.launch_pieces, narrow = FwdGeom<N>::kTE, wide = FwdGeom<N, true>::kTE;
       if (rows * ((p.ED + narrow - 1) / narrow) > sms && rows * ((p.ED + wide - 1) / wide) <= sms) return tma_launch_tile<T, N, true>(p, st);
     }
   }
@@ -807,4 +877,55 @@ extern "C" int mb200_sscan_fwd_carry(const void* x, const void* delta, const flo
                                      int64_t b_sb, int64_t b_sl, int dtype, int flags, void* stream) {
   return mb200_sscan_fwd_carry_pieces(x, delta, A, Bm, delta_bias, h_out, p_out, B, L, ED, N, x_sb, x_sl, d_sb, d_sl, b_sb, b_sl, dtype, flags,
                                       1, 0, stream);
+}
+
+// The pieces of cut sequences come from the carry pass in front of the scan, both in one call.
+extern "C" int64_t mb200_packed_pieces(int64_t rows, int64_t sequences, int64_t piece_len) {
+  return piece_len > 0 ? packed_items(rows, sequences, piece_len) : 0;
+}
+extern "C" int64_t mb200_packed_saved_states(int64_t rows, int64_t sequences) { return packed_chunks(rows, sequences, kChunk); }
+
+extern "C" int mb200_sscan_packed_fwd(const mb200_packed* seqs, const void* x, const void* delta, const void* z, const float* A, const void* Bm,
+                                      const void* Cm, const float* D, const float* delta_bias, float* states, void* y, float* carries,
+                                      float* pieces, int64_t ED, int N, int64_t x_sl, int64_t d_sl, int64_t z_sl, int64_t b_sl,
+                                      int64_t c_sl, int64_t y_sl, int64_t piece_len, int dtype, int flags, void* stream) {
+  if (const int rc = packed_check(seqs)) return rc;
+  if (ED < 0 || piece_len < 0 || piece_len % kTile) return MB200_EINVAL;
+  if (dtype != MB200_F32 && dtype != MB200_BF16) return MB200_EDTYPE;
+  if (N != 8 && N != 16 && N != 32 && N != 64) return MB200_ENSTATE;
+  if (seqs->rows == 0 || ED == 0) return MB200_OK;
+  if (!x || !delta || !A || !Bm || !Cm || !y) return MB200_EINVAL;
+  if ((flags & MB200_DELTA_SOFTPLUS) && !delta_bias) return MB200_EINVAL;
+  if (seqs->slots && !states) return MB200_EINVAL;
+  if (flags & MB200_REVERSE) return MB200_EUNSUPPORTED;
+  if (!aligned16(states) || !aligned16(carries) || !aligned16(pieces)) return MB200_EALIGN;
+  if (piece_len && (!pieces || N != 16)) return MB200_EINVAL;
+  SscanFwdParams p{};
+  p.x = x; p.delta = delta; p.z = z; p.A = A; p.Bm = Bm; p.Cm = Cm; p.D = D;
+  p.delta_bias = delta_bias; p.h0 = p.hT = states; p.y = y; p.carries = carries;
+  p.B = 1; p.L = seqs->rows; p.ED = ED;
+  p.x_sl = x_sl; p.d_sl = d_sl; p.z_sl = z_sl; p.b_sl = b_sl; p.c_sl = c_sl; p.y_sl = y_sl;
+  p.flags = flags & (MB200_DELTA_SOFTPLUS | MB200_GENERAL_DECAY | MB200_PAIRED_STATES);
+  p.seqs = packed_of(*seqs, piece_len);
+  if (!states) p.seqs.slots = nullptr;
+  p.pieceP = pieces;
+  p.pieceS = pieces ? pieces + packed_items(seqs->rows, seqs->sequences, piece_len) * ED * N : nullptr;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int es = dtype == MB200_F32 ? 4 : 2;
+  if (tma_path_ok(p, N, es)) {
+    auto launch = [&](const SscanFwdParams& q) { return dtype == MB200_F32 ? tma_launch_t<float>(q, N, st) : tma_launch_t<__nv_bfloat16>(q, N, st); };
+    int rc = MB200_OK;
+    if (piece_len) {
+      SscanFwdParams c = p;
+      c.y = nullptr; c.z = nullptr; c.Cm = Bm; c.c_sl = b_sl; c.carries = nullptr;
+      rc = launch(c);
+    }
+    if (rc == MB200_OK) rc = launch(p);
+    if (rc <= 0) return rc;                        // launched (0) or failed hard (< 0)
+  }
+  if (piece_len) return MB200_EUNSUPPORTED;
+  const int kv = dtype == MB200_F32 ? 4 : 8;
+  bool vec = ED % kv == 0 && aligned16(x) && aligned16(delta) && aligned16(z) && aligned16(y) && aligned16(Bm) && aligned16(Cm);
+  for (int64_t s : {x_sl, d_sl, y_sl, b_sl, c_sl, z ? z_sl : 0}) vec = vec && s % kv == 0;
+  return dtype == MB200_F32 ? generic_launch_t<float>(p, N, vec, st) : generic_launch_t<__nv_bfloat16>(p, N, vec, st);
 }

@@ -63,7 +63,8 @@ __device__ __forceinline__ int yp_slot(int t, int e_l) {
   return e_l;
 }
 
-template <typename T, int N, int KV>
+// kPacked: a CTA's row of the batch is a sequence of `p.seqs`, with its state in a slot of the pool.
+template <typename T, int N, int KV, bool kPacked = false>
 __global__ void __launch_bounds__(kGenThreads, 3)
 sscan_fwd_generic_kernel(const SscanFwdParams p) {
   using G = SscanGeom<N>;
@@ -83,12 +84,25 @@ sscan_fwd_generic_kernel(const SscanFwdParams p) {
 
   const int tid = threadIdx.x;
   const int64_t e0 = int64_t(blockIdx.x) * kTE;
-  const int64_t b = blockIdx.y;
+  const int64_t b = kPacked ? 0 : blockIdx.y;
+  PackedItem item{};
+  if constexpr (kPacked) item = packed_item<kGenThreads>(p.seqs, int(blockIdx.y), threadIdx.x);
+  const int64_t row0 = kPacked ? item.lo : 0, L = kPacked ? item.hi - item.lo : p.L;
   const int cols_ok = int(min64(kTE, p.ED - e0));
   const bool softplus = (p.flags & MB200_DELTA_SOFTPLUS) != 0;
   const bool has_y = p.y != nullptr;
   const bool has_z = p.z != nullptr;
-  const int64_t ntiles = (p.L + kTT - 1) / kTT;
+  const int64_t ntiles = (L + kTT - 1) / kTT;
+  int64_t slot = b;
+  bool enters = p.h0 != nullptr, leaves = p.hT != nullptr;
+  if constexpr (kPacked) {
+    if (item.seq == p.seqs.sequences)
+      zero_rows<T, kGenThreads>(static_cast<T*>(p.y) + e0, p.y_sl, item.lo, item.hi, cols_ok, tid);
+    if (item.seq == p.seqs.sequences || L == 0) return;
+    slot = p.seqs.slot(item.seq);
+    leaves = slot >= 0;
+    enters = leaves && p.seqs.resumes(item.seq);
+  }
 
   if (tid == 0) {
     mbar_init(&bars[0], kGenProducers); mbar_init(&bars[1], kGenProducers);
@@ -106,14 +120,14 @@ sscan_fwd_generic_kernel(const SscanFwdParams p) {
     const int e_l = tid / kLPE, q = tid % kLPE;
     const int64_t e = e0 + e_l;
     const bool e_ok = e < p.ED;
-    const int64_t nchunks = (p.L + kChunk - 1) / kChunk;
+    const int64_t chunk0 = kPacked ? item.begin / kChunk + item.seq : b * ((p.L + kChunk - 1) / kChunk);
     float2 A2lo, A2hi, hlo, hhi;
     {
       float a4[4], h4[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         a4[j] = e_ok ? p.A[e * N + 4 * q + j] * kLog2e : 0.f;
-        h4[j] = (e_ok && p.h0) ? p.h0[(b * p.ED + e) * N + 4 * q + j] : 0.f;
+        h4[j] = (e_ok && enters) ? p.h0[(slot * p.ED + e) * N + 4 * q + j] : 0.f;
       }
       A2lo = make_float2(a4[0], a4[1]); A2hi = make_float2(a4[2], a4[3]);
       hlo = make_float2(h4[0], h4[1]); hhi = make_float2(h4[2], h4[3]);
@@ -135,8 +149,8 @@ sscan_fwd_generic_kernel(const SscanFwdParams p) {
       float* yp = s_yp + buf * kTT * kConsumers;
 #pragma unroll
       for (int t = 0; t < kTT; ++t) {
-        if ((t % kChunk) == 0 && p.carries && e_ok && t0 + t < p.L) {
-          store_states(p.carries + (b * nchunks + (t0 + t) / kChunk) * p.ED * N, (p.flags & MB200_PAIRED_STATES) != 0, p.ED, N, e, q,
+        if ((t % kChunk) == 0 && p.carries && e_ok && t0 + t < L) {
+          store_states(p.carries + (chunk0 + (t0 + t) / kChunk) * p.ED * N, (p.flags & MB200_PAIRED_STATES) != 0, p.ED, N, e, q,
                        make_float4(hlo.x, hlo.y, hhi.x, hhi.y));
         }
         const float2 o = op[t * kTE + ((t & 1) ? op_off1 : op_off0)];   // {delta, delta*x}
@@ -156,8 +170,8 @@ sscan_fwd_generic_kernel(const SscanFwdParams p) {
       }
       mbar_arrive(&bars[2 + buf]);
     }
-    if (p.hT && e_ok) {
-      float4* dst = reinterpret_cast<float4*>(p.hT + (b * p.ED + e) * N + 4 * q);
+    if (leaves && e_ok) {
+      float4* dst = reinterpret_cast<float4*>(p.hT + (slot * p.ED + e) * N + 4 * q);
       *dst = make_float4(hlo.x, hlo.y, hhi.x, hhi.y);
     }
   } else {
@@ -169,18 +183,18 @@ sscan_fwd_generic_kernel(const SscanFwdParams p) {
     using AMap = typename ActRegs::Map;
     constexpr int kPT = AMap::kPerThread;
 
-    const T* gx = static_cast<const T*>(p.x) + b * p.x_sb + e0;
-    const T* gd = static_cast<const T*>(p.delta) + b * p.d_sb + e0;
-    const T* gz = has_z ? static_cast<const T*>(p.z) + b * p.z_sb + e0 : nullptr;
-    const T* gB = static_cast<const T*>(p.Bm) + b * p.b_sb;
-    const T* gC = static_cast<const T*>(p.Cm) + b * p.c_sb;
-    T* gy = has_y ? static_cast<T*>(p.y) + b * p.y_sb + e0 : nullptr;
+    const T* gx = static_cast<const T*>(p.x) + b * p.x_sb + row0 * p.x_sl + e0;
+    const T* gd = static_cast<const T*>(p.delta) + b * p.d_sb + row0 * p.d_sl + e0;
+    const T* gz = has_z ? static_cast<const T*>(p.z) + b * p.z_sb + row0 * p.z_sl + e0 : nullptr;
+    const T* gB = static_cast<const T*>(p.Bm) + b * p.b_sb + row0 * p.b_sl;
+    const T* gC = static_cast<const T*>(p.Cm) + b * p.c_sb + row0 * p.c_sl;
+    T* gy = has_y ? static_cast<T*>(p.y) + b * p.y_sb + row0 * p.y_sl + e0 : nullptr;
 
     ActRegs rx, rd, rz;
     BcRegs rB, rC;
     auto fetch = [&](int64_t kt) {
       const int64_t t0 = kt * kTT;
-      const int rows_ok = int(min64(kTT, p.L - t0));
+      const int rows_ok = int(min64(kTT, L - t0));
       rx.load(gx + t0 * p.x_sl, p.x_sl, rows_ok, cols_ok, pt);
       rd.load(gd + t0 * p.d_sl, p.d_sl, rows_ok, cols_ok, pt);
       if (has_z) rz.load(gz + t0 * p.z_sl, p.z_sl, rows_ok, cols_ok, pt);
@@ -190,7 +204,7 @@ sscan_fwd_generic_kernel(const SscanFwdParams p) {
     // convert the fetched tile and publish it in buffer kt & 1
     auto commit = [&](int64_t kt) {
       const int buf = int(kt & 1);
-      const int rows_ok = int(min64(kTT, p.L - kt * kTT));
+      const int rows_ok = int(min64(kTT, L - kt * kTT));
       float2* tile = s_op + buf * kTT * kTE;
 #pragma unroll
       for (int i = 0; i < kPT; ++i) {
@@ -202,7 +216,7 @@ sscan_fwd_generic_kernel(const SscanFwdParams p) {
           const bool ok = rr < rows_ok && cc + k < cols_ok;
           float dv = Elem<T>::to_f(rd.r[i].v[k]);
           const float xv = Elem<T>::to_f(rx.r[i].v[k]);
-          if (softplus) dv = ok ? softplus_fast(dv + s_bias[cc + k]) : 0.f;
+          if (softplus) dv = ok ? (kPacked ? softplus_near(dv + s_bias[cc + k]) : softplus_fast(dv + s_bias[cc + k])) : 0.f;
           v[k] = make_float2(dv, dv * xv);
         }
         if constexpr (KV % 2 == 0) {
@@ -225,7 +239,7 @@ sscan_fwd_generic_kernel(const SscanFwdParams p) {
     auto epilogue = [&](int64_t kt) {
       const int buf = int(kt & 1);
       const int64_t t0 = kt * kTT;
-      const int rows_ok = int(min64(kTT, p.L - t0));
+      const int rows_ok = int(min64(kTT, L - t0));
       const float* yp = s_yp + buf * kTT * kConsumers;
 #pragma unroll
       for (int i = 0; i < kPT; ++i) {
@@ -275,11 +289,11 @@ template <typename T, int N>
 int generic_launch_n(const SscanFwdParams& p, bool vec, cudaStream_t st) {
   using G = SscanGeom<N>;
   using S = GenFwdSmem<T, N>;
-  dim3 grid(unsigned((p.ED + G::kTE - 1) / G::kTE), unsigned(p.B));
+  const bool packed = p.seqs.rows > 0;
+  dim3 grid(unsigned((p.ED + G::kTE - 1) / G::kTE), unsigned(packed ? p.seqs.sequences + 1 : p.B));
   constexpr int KV = Elem<T>::kVec;
-  auto kv = sscan_fwd_generic_kernel<T, N, KV>;
-  auto k1 = sscan_fwd_generic_kernel<T, N, 1>;
-  auto k = vec ? kv : k1;
+  auto k = packed ? (vec ? sscan_fwd_generic_kernel<T, N, KV, true> : sscan_fwd_generic_kernel<T, N, 1, true>)
+                  : (vec ? sscan_fwd_generic_kernel<T, N, KV> : sscan_fwd_generic_kernel<T, N, 1>);
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess)
     return MB200_ELAUNCH;
   k<<<grid, kGenThreads, S::kBytes, st>>>(p);

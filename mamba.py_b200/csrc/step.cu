@@ -36,14 +36,16 @@ struct Param {
 // do better with A.  (Several rows per CTA, parameters fetched once for all of them, measured slower: 34.2 us for two rows
 // and 35.6 for four against 31.5 at B 256, ED 5120: the registers cost more resident CTAs than the loads do.)
 // kF32: every parameter is float32 (the type test costs the streaming kernel registers and 4 us of 32).
-template <typename T, int N, bool kVecBC, bool kLogA, bool kF32>
+// kSlots: row b's state is entry slots[b] of a pool of n_slots, h_in and h_out alike; a row with a slot outside it gives zero and
+// touches nothing.
+template <typename T, int N, bool kVecBC, bool kLogA, bool kF32, bool kSlots = false>
 __global__ void __launch_bounds__(kStepThreads)
 ssm_step_kernel(const T* __restrict__ x, const T* __restrict__ delta, const T* __restrict__ z,
                 const Param A_, const T* __restrict__ Bm, const T* __restrict__ Cm,
                 const Param D_, const Param delta_bias_,
                 const float* __restrict__ h_in, float* __restrict__ h_out, T* __restrict__ y,
                 int64_t ED, int64_t x_sb, int64_t d_sb, int64_t z_sb, int64_t b_sb,
-                int64_t c_sb, int64_t y_sb, int flags) {
+                int64_t c_sb, int64_t y_sb, int flags, const int64_t* __restrict__ slots, int64_t n_slots) {
   constexpr int kSPL = MB200_STEP_SPL < N ? MB200_STEP_SPL : N;   // states per lane
   constexpr int kV = kSPL / 4;                                    // float4 per lane
   constexpr int kLPE = N / kSPL;                                  // lanes per channel
@@ -55,12 +57,16 @@ ssm_step_kernel(const T* __restrict__ x, const T* __restrict__ delta, const T* _
   const int q = tid % kLPE;
   const int64_t e = int64_t(blockIdx.x) * kEPB + tid / kLPE;
   const bool ok = e < ED;
-  const int64_t b = blockIdx.y;
+  const int64_t b = blockIdx.y, hb = kSlots ? __ldg(slots + b) : b;
   float yv = 0.f, xv = 0.f;
+  if (kSlots && (hb < 0 || hb >= n_slots)) {
+    if (ok && q == 0) y[b * y_sb + e] = Elem<T>::from_f(0.f);
+    return;
+  }
   if (ok) {
     // the state is the only large stream: get it moving first, everything else is small
     float4 hv[kV];
-    const float4* hp = reinterpret_cast<const float4*>(h_in + (b * ED + e) * N + kSPL * q);
+    const float4* hp = reinterpret_cast<const float4*>(h_in + (hb * ED + e) * N + kSPL * q);
 #pragma unroll
     for (int v = 0; v < kV; ++v) hv[v] = h_in ? __ldcs(hp + v) : make_float4(0.f, 0.f, 0.f, 0.f);
     float Av[kSPL];
@@ -95,11 +101,14 @@ ssm_step_kernel(const T* __restrict__ x, const T* __restrict__ delta, const T* _
     }
     xv = Elem<T>::to_f(x[b * x_sb + e]);
     float dv = Elem<T>::to_f(delta[b * d_sb + e]);
-    if (flags & MB200_DELTA_SOFTPLUS) dv = softplus_fast(dv + (kF32 ? delta_bias[e] : delta_bias_.at(e)));
+    if (flags & MB200_DELTA_SOFTPLUS) {
+      dv += kF32 ? delta_bias[e] : delta_bias_.at(e);
+      dv = kSlots ? softplus_near(dv) : softplus_fast(dv);
+    }
     const float dxs = dv * xv, d2s = dv * kLog2e;
     const float2 dx = make_float2(dxs, dxs), d2 = make_float2(d2s, d2s);
     float2 y2 = make_float2(0.f, 0.f);
-    float4* op = reinterpret_cast<float4*>(h_out + (b * ED + e) * N + kSPL * q);
+    float4* op = reinterpret_cast<float4*>(h_out + (hb * ED + e) * N + kSPL * q);
 #pragma unroll
     for (int v = 0; v < kV; ++v) {
       // packed f32x2 arithmetic: two states per instruction (the decays stay scalar ex2)
@@ -126,16 +135,20 @@ ssm_step_kernel(const T* __restrict__ x, const T* __restrict__ delta, const T* _
 }
 
 // xc = silu(sum_k w[e,k]*win[k] + bias[e]) with win = [conv_in[b,e,:], xin[b,e]]; conv_out = win[1:].
-template <typename T>
+template <typename T, bool kSlots = false>
 __global__ void conv_step_kernel(const T* __restrict__ xin, const T* __restrict__ conv_in,
                                  const Param w, const Param bias,
                                  T* __restrict__ xc, T* __restrict__ conv_out,
-                                 int64_t ED, int K, int64_t x_sb) {
+                                 int64_t ED, int K, int64_t x_sb, const int64_t* __restrict__ slots, int64_t n_slots) {
   const int64_t e = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int64_t b = blockIdx.y;
+  const int64_t b = blockIdx.y, wb = kSlots ? __ldg(slots + b) : b;
   if (e >= ED) return;
-  const T* ci = conv_in + (b * ED + e) * (K - 1);
-  T* co = conv_out + (b * ED + e) * (K - 1);
+  if (kSlots && (wb < 0 || wb >= n_slots)) {
+    xc[b * ED + e] = Elem<T>::from_f(0.f);
+    return;
+  }
+  const T* ci = conv_in + (wb * ED + e) * (K - 1);
+  T* co = conv_out + (wb * ED + e) * (K - 1);
   const float xn = Elem<T>::to_f(xin[b * x_sb + e]);
   float acc = bias.p ? bias.at(e) : 0.f;
   float win[8];
@@ -149,21 +162,29 @@ __global__ void conv_step_kernel(const T* __restrict__ xin, const T* __restrict_
 // Same for the common d_conv = 4: a thread owns 4 neighbouring channels, so the 3-wide windows of
 // those channels (12 contiguous elements) and the new inputs move as 8- or 16-byte vectors.  Rows of blocks past the batch
 // work on `jobs`, the parameter conversions of the state update that follows: a launch of their own cost 2.3 us and its gap.
-template <typename T>
+template <typename T, bool kSlots = false>
 __global__ void __launch_bounds__(256)
 conv_step_k4_kernel(const T* __restrict__ xin, const T* __restrict__ conv_in, const Param w,
                     const Param bias, T* __restrict__ xc, T* __restrict__ conv_out,
-                    int64_t B, int64_t ED, int64_t x_sb, const __grid_constant__ Jobs<kStepJobs> jobs) {
+                    int64_t B, int64_t ED, int64_t x_sb, const __grid_constant__ Jobs<kStepJobs> jobs,
+                    const int64_t* __restrict__ slots, int64_t n_slots) {
   if (blockIdx.y >= B) {
     const int block = int((blockIdx.y - B) * gridDim.x + blockIdx.x);
     if (block < jobs.first_block[jobs.n]) convert_block(jobs, block);
     return;
   }
   const int64_t e = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) * 4;
-  const int64_t b = blockIdx.y;
+  const int64_t b = blockIdx.y, wb = kSlots ? __ldg(slots + b) : b;
   if (e >= ED) return;
-  const Vec4<T>* ci = reinterpret_cast<const Vec4<T>*>(conv_in + (b * ED + e) * 3);
-  Vec4<T>* co = reinterpret_cast<Vec4<T>*>(conv_out + (b * ED + e) * 3);
+  if (kSlots && (wb < 0 || wb >= n_slots)) {
+    Vec4<T> none;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) none.v[c] = Elem<T>::from_f(0.f);
+    *reinterpret_cast<Vec4<T>*>(xc + b * ED + e) = none;
+    return;
+  }
+  const Vec4<T>* ci = reinterpret_cast<const Vec4<T>*>(conv_in + (wb * ED + e) * 3);
+  Vec4<T>* co = reinterpret_cast<Vec4<T>*>(conv_out + (wb * ED + e) * 3);
   const Vec4<T> w0 = ci[0], w1 = ci[1], w2 = ci[2];            // 12 window values of 4 channels
   const Vec4<T> xn = *reinterpret_cast<const Vec4<T>*>(xin + b * x_sb + e);
   T win[12] = {w0.v[0], w0.v[1], w0.v[2], w0.v[3], w1.v[0], w1.v[1], w1.v[2], w1.v[3],
@@ -280,14 +301,14 @@ template <typename T>
 static int ssm_step_t(const void* x, const void* delta, const void* z, Param A, const void* Bm, const void* Cm, Param D,
                       Param delta_bias, const float* h_in, float* h_out, void* y, int64_t B, int64_t ED, int N,
                       int64_t x_sb, int64_t d_sb, int64_t z_sb, int64_t b_sb, int64_t c_sb,
-                      int64_t y_sb, int flags, bool log_A, cudaStream_t st) {
+                      int64_t y_sb, int flags, bool log_A, const int64_t* slots, int64_t n_slots, cudaStream_t st) {
   const bool vec_bc = (reinterpret_cast<uintptr_t>(Bm) % (4 * sizeof(T)) == 0) &&
                       (reinterpret_cast<uintptr_t>(Cm) % (4 * sizeof(T)) == 0) && b_sb % 4 == 0 && c_sb % 4 == 0;
   const bool all_f32 = A.dtype == MB200_F32 && D.dtype == MB200_F32 && delta_bias.dtype == MB200_F32;
 #define MB200_STEP_LAUNCH(NN, V, LOGA, F)                                                       \
-  ssm_step_kernel<T, NN, V, LOGA, F><<<grid, kStepThreads, 0, st>>>(                            \
+  (slots ? ssm_step_kernel<T, NN, V, LOGA, F, true> : ssm_step_kernel<T, NN, V, LOGA, F, false>)<<<grid, kStepThreads, 0, st>>>( \
       (const T*)x, (const T*)delta, (const T*)z, A, (const T*)Bm, (const T*)Cm, D, delta_bias, \
-      h_in, h_out, (T*)y, ED, x_sb, d_sb, z_sb, b_sb, c_sb, y_sb, flags)
+      h_in, h_out, (T*)y, ED, x_sb, d_sb, z_sb, b_sb, c_sb, y_sb, flags, slots, n_slots)
 #define MB200_STEP(NN)                                                                          \
   {                                                                                             \
     constexpr int epb = kStepThreads / (NN / (MB200_STEP_SPL < NN ? MB200_STEP_SPL : NN));      \
@@ -310,12 +331,12 @@ static int ssm_step_t(const void* x, const void* delta, const void* z, Param A, 
 #undef MB200_STEP_LAUNCH
 }
 
-extern "C" int mb200_ssm_step_params(const void* x, const void* delta, const void* z, const void* A, int A_dtype, int A_is_log,
+static int ssm_step_any(const void* x, const void* delta, const void* z, const void* A, int A_dtype, int A_is_log,
                                      const void* Bm, const void* Cm, const void* D, int D_dtype, const void* delta_bias,
                                      int bias_dtype, const float* h_in, float* h_out, void* y,
                                      int64_t B, int64_t ED, int N, int64_t x_sb, int64_t d_sb,
                                      int64_t z_sb, int64_t b_sb, int64_t c_sb, int64_t y_sb, int dtype,
-                                     int flags, void* stream) {
+                                     int flags, const int64_t* slots, int64_t n_slots, void* stream) {
   if (B < 0 || ED < 0) return MB200_EINVAL;
   if (dtype != MB200_F32 && dtype != MB200_BF16) return MB200_EDTYPE;
   for (int d : {A_dtype, D_dtype, bias_dtype})
@@ -330,9 +351,30 @@ extern "C" int mb200_ssm_step_params(const void* x, const void* delta, const voi
   const Param pA{A, A_dtype}, pD{D, D_dtype}, pb{delta_bias, bias_dtype};
   return dtype == MB200_F32
              ? ssm_step_t<float>(x, delta, z, pA, Bm, Cm, pD, pb, h_in, h_out, y, B, ED, N, x_sb, d_sb, z_sb, b_sb, c_sb, y_sb, flags,
-                                 A_is_log != 0, st)
+                                 A_is_log != 0, slots, n_slots, st)
              : ssm_step_t<__nv_bfloat16>(x, delta, z, pA, Bm, Cm, pD, pb, h_in, h_out, y, B, ED, N, x_sb, d_sb, z_sb, b_sb, c_sb, y_sb,
-                                         flags, A_is_log != 0, st);
+                                         flags, A_is_log != 0, slots, n_slots, st);
+}
+
+extern "C" int mb200_ssm_step_params(const void* x, const void* delta, const void* z, const void* A, int A_dtype, int A_is_log,
+                                     const void* Bm, const void* Cm, const void* D, int D_dtype, const void* delta_bias,
+                                     int bias_dtype, const float* h_in, float* h_out, void* y,
+                                     int64_t B, int64_t ED, int N, int64_t x_sb, int64_t d_sb,
+                                     int64_t z_sb, int64_t b_sb, int64_t c_sb, int64_t y_sb, int dtype,
+                                     int flags, void* stream) {
+  return ssm_step_any(x, delta, z, A, A_dtype, A_is_log, Bm, Cm, D, D_dtype, delta_bias, bias_dtype, h_in, h_out, y, B, ED, N, x_sb, d_sb, z_sb,
+                      b_sb, c_sb, y_sb, dtype, flags, nullptr, 0, stream);
+}
+
+extern "C" int mb200_ssm_step_slots(const void* x, const void* delta, const void* z, const void* A, int A_dtype, int A_is_log,
+                                    const void* Bm, const void* Cm, const void* D, int D_dtype, const void* delta_bias,
+                                    int bias_dtype, float* states, const int64_t* slots, int64_t n_slots, void* y,
+                                    int64_t B, int64_t ED, int N, int64_t x_sb, int64_t d_sb,
+                                    int64_t z_sb, int64_t b_sb, int64_t c_sb, int64_t y_sb, int dtype,
+                                    int flags, void* stream) {
+  if (n_slots < 0 || (B > 0 && !slots)) return MB200_EINVAL;
+  return ssm_step_any(x, delta, z, A, A_dtype, A_is_log, Bm, Cm, D, D_dtype, delta_bias, bias_dtype, states, states, y, B, ED, N, x_sb, d_sb,
+                      z_sb, b_sb, c_sb, y_sb, dtype, flags, slots, n_slots, stream);
 }
 
 extern "C" int mb200_ssm_step(const void* x, const void* delta, const void* z, const float* A,
@@ -345,9 +387,10 @@ extern "C" int mb200_ssm_step(const void* x, const void* delta, const void* z, c
                                d_sb, z_sb, b_sb, c_sb, y_sb, dtype, flags, stream);
 }
 
-extern "C" int mb200_conv_step_convert(const void* xin, const void* conv_in, const void* w, int w_dtype,
+static int conv_step_any(const void* xin, const void* conv_in, const void* w, int w_dtype,
                                        const void* bias, int bias_dtype, void* xc, void* conv_out, int64_t B, int64_t ED,
-                                       int K, int64_t x_sb, int dtype, const mb200_convert_job* jobs, int n_jobs, void* stream) {
+                                       int K, int64_t x_sb, int dtype, const mb200_convert_job* jobs, int n_jobs,
+                         const int64_t* slots, int64_t n_slots, void* stream) {
   if (B < 0 || ED < 0 || K < 1) return MB200_EINVAL;
   if (K > 8) return MB200_ETOOBIG;
   for (int d : {dtype, w_dtype, bias_dtype})
@@ -368,25 +411,36 @@ extern "C" int mb200_conv_step_convert(const void* xin, const void* conv_in, con
     const bool along = B + extra <= 65535;
     if (along) g4.y += unsigned(extra);
     else if (const int rc = mb200_convert(jobs, n_jobs, stream)) return rc;
-    if (dtype == MB200_F32)
-      conv_step_k4_kernel<float><<<g4, 256, 0, st>>>((const float*)xin, (const float*)conv_in, pw, pb,
-                                                     (float*)xc, (float*)conv_out, B, ED, x_sb, all);
-    else
-      conv_step_k4_kernel<__nv_bfloat16><<<g4, 256, 0, st>>>(
-          (const __nv_bfloat16*)xin, (const __nv_bfloat16*)conv_in, pw, pb, (__nv_bfloat16*)xc,
-          (__nv_bfloat16*)conv_out, B, ED, x_sb, all);
+#define MB200_CONV_STEP(TT)                                                                                                             \
+  (slots ? conv_step_k4_kernel<TT, true> : conv_step_k4_kernel<TT, false>)<<<g4, 256, 0, st>>>((const TT*)xin, (const TT*)conv_in, pw, pb, \
+                                                                                             (TT*)xc, (TT*)conv_out, B, ED, x_sb, all, slots, n_slots)
+    if (dtype == MB200_F32) MB200_CONV_STEP(float);
+    else MB200_CONV_STEP(__nv_bfloat16);
+#undef MB200_CONV_STEP
     return check_launch();
   }
   if (const int rc = mb200_convert(jobs, n_jobs, stream)) return rc;
   dim3 grid(unsigned((ED + 255) / 256), unsigned(B));
-  if (dtype == MB200_F32)
-    conv_step_kernel<float><<<grid, 256, 0, st>>>((const float*)xin, (const float*)conv_in, pw, pb,
-                                                  (float*)xc, (float*)conv_out, ED, K, x_sb);
-  else
-    conv_step_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(
-        (const __nv_bfloat16*)xin, (const __nv_bfloat16*)conv_in, pw, pb, (__nv_bfloat16*)xc,
-        (__nv_bfloat16*)conv_out, ED, K, x_sb);
+#define MB200_CONV_STEP(TT)                                                                                                       \
+  (slots ? conv_step_kernel<TT, true> : conv_step_kernel<TT, false>)<<<grid, 256, 0, st>>>((const TT*)xin, (const TT*)conv_in, pw, pb, \
+                                                                                         (TT*)xc, (TT*)conv_out, ED, K, x_sb, slots, n_slots)
+  if (dtype == MB200_F32) MB200_CONV_STEP(float);
+  else MB200_CONV_STEP(__nv_bfloat16);
+#undef MB200_CONV_STEP
   return check_launch();
+}
+
+extern "C" int mb200_conv_step_convert(const void* xin, const void* conv_in, const void* w, int w_dtype,
+                                       const void* bias, int bias_dtype, void* xc, void* conv_out, int64_t B, int64_t ED,
+                                       int K, int64_t x_sb, int dtype, const mb200_convert_job* jobs, int n_jobs, void* stream) {
+  return conv_step_any(xin, conv_in, w, w_dtype, bias, bias_dtype, xc, conv_out, B, ED, K, x_sb, dtype, jobs, n_jobs, nullptr, 0, stream);
+}
+
+extern "C" int mb200_conv_step_slots(const void* xin, void* windows, const int64_t* slots, int64_t n_slots, const void* w, int w_dtype,
+                                     const void* bias, int bias_dtype, void* xc, int64_t B, int64_t ED, int K, int64_t x_sb, int dtype,
+                                     void* stream) {
+  if (n_slots < 0 || (B > 0 && !slots)) return MB200_EINVAL;
+  return conv_step_any(xin, windows, w, w_dtype, bias, bias_dtype, xc, windows, B, ED, K, x_sb, dtype, nullptr, 0, slots, n_slots, stream);
 }
 
 extern "C" int mb200_conv_step(const void* xin, const void* conv_in, const float* w,

@@ -48,6 +48,25 @@ def selective_scan_fn(x, delta, A, B, C, D=None, z=None, delta_bias=None, h0=Non
     return _host().selective_scan(x, delta, A, B, C, D, z, delta_bias, h0, return_last_state, reverse, subshards)
 
 
+def selective_scan_packed(x, delta, A, B, C, D=None, z=None, delta_bias=None, *, cu_seqlens, states=None, slots=None, resume=None,
+                          max_length=None, piece_length=None):
+    """`selective_scan_fn` over sequences of different lengths laid end to end, without padding.
+
+    x, delta, z : (T, ED)   B, C : (T, N)   cu_seqlens : (R + 1,) int32 or int64 on the device, 0 first, where each sequence begins and
+    the last one ends; rows behind that (padding of a captured batch) give zeros.  Returns y (T, ED).
+
+    For training on packed documents the gradients of all eight inputs are there, and nothing crosses a border.  For serving, `states`
+    (S, ED, N) float32 is a pool that is updated in place and `slots` (R,) says which entry is whose: each sequence leaves its last state
+    there, and starts from what is there where `resume` (R,) bool says so (from zero otherwise), which is how a prompt is read in chunks.  A
+    slot outside the pool is nobody's: no state is read or left.  Slots of one call must differ.  A sequence of no rows changes nothing.
+
+    cu_seqlens, slots and resume stay on the device: a captured call can be replayed with other contents.  `max_length` is a bound on the
+    lengths, if the caller has one; a sequence that is much longer than the others is then cut into pieces that are scanned side by side
+    only where it pays (d_state 16, tensors on the 16-byte grid).  It guides this choice alone.  `piece_length` (a multiple of 16) cuts there
+    instead, 0 nowhere."""
+    return _host().selective_scan_packed(x, delta, A, B, C, D, z, delta_bias, cu_seqlens, states, slots, resume, max_length, piece_length)
+
+
 # ----------------------------------------------------------------- MambaBlock method drop-ins
 
 def selective_scan(self, x, delta, A, B, C, D):
@@ -60,23 +79,28 @@ def selective_scan_seq(self, x, delta, A, B, C, D):
     return selective_scan_fn(x, delta, A, B, C, D)
 
 
-def ssm_step_fn(x, h, delta, A, B, C, D=None, z=None, delta_bias=None, inplace=False):
+def ssm_step_fn(x, h, delta, A, B, C, D=None, z=None, delta_bias=None, inplace=False, slots=None):
     """One decode step on projected inputs.  x, delta, z: (B, ED); B, C: (B, N); h: (B, ED, N) or None.
 
     Returns (y, h_new); h_new is a fresh float32 tensor (the reference also returns a new one,
     mambapy/mamba.py:408).  `inplace=True` (opt-in, for decode loops that own their cache)
-    overwrites a float32 contiguous `h` instead and returns it."""
-    return _host().ssm_step(x, h, delta, A, B, C, D, z, delta_bias, inplace)
+    overwrites a float32 contiguous `h` instead and returns it.
+
+    With `slots` (B,) `h` is a pool (S, ED, N), float32 and contiguous, whose entry slots[b] is row b's state, always updated in place.  A
+    row with a slot outside the pool gives zeros and updates nothing (padding of a captured batch).  Slots of one call must differ."""
+    return _host().ssm_step(x, h, delta, A, B, C, D, z, delta_bias, inplace, slots)
 
 
-def conv_step_fn(x, inputs, weight, bias, inplace=False):
+def conv_step_fn(x, inputs, weight, bias, inplace=False, slots=None):
     """Conv-window part of a decode step (mambapy/mamba.py:366-369, :379).
 
     x: (B, ED) new pre-conv input; inputs: (B, ED, d_conv-1) cached window;
     weight: (ED, 1, d_conv) depthwise filter; bias: (ED) or None.
     Returns (silu(conv(x)), new window).  The window is a fresh tensor unless `inplace=True`
-    (opt-in), which shifts a contiguous window of the activation dtype in place."""
-    return _host().conv_step(x, inputs, weight, bias, inplace)
+    (opt-in), which shifts a contiguous window of the activation dtype in place.
+
+    With `slots` (B,) `inputs` is a pool (S, ED, d_conv-1) of the activation dtype, as for `ssm_step_fn`."""
+    return _host().conv_step(x, inputs, weight, bias, inplace, slots)
 
 
 def causal_conv1d_silu(x, weight, bias=None):
@@ -84,6 +108,14 @@ def causal_conv1d_silu(x, weight, bias=None):
 
     x: (B, L, ED); weight: (ED, 1, 4) as nn.Conv1d(groups=ED) holds it; bias: (ED) or None."""
     return _host().conv1d_silu(x, weight, bias)
+
+
+def causal_conv1d_silu_packed(x, weight, bias=None, *, cu_seqlens, windows=None, slots=None, resume=None):
+    """`causal_conv1d_silu` over sequences of different lengths laid end to end: x (T, ED), cu_seqlens as for `selective_scan_packed`.
+
+    With gradients for training; for serving `windows` (S, ED, 3), of x's dtype, is a pool whose entry slots[r] sequence r leaves its last
+    three inputs in, and starts from where `resume` says so."""
+    return _host().conv1d_silu_packed(x, weight, bias, cu_seqlens, windows, slots, resume)
 
 
 def rms_norm(x, weight=None, eps=1e-5):
