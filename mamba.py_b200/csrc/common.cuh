@@ -101,19 +101,28 @@ __device__ __forceinline__ float2 softplus_fast2(float2 x) {
 // softplus to within 3e-7 of its value (arguments above -8; the exponential's argument is rounded): max(x, 0) + log1p(e^-|x|), with
 // log1p(u) = u q(u) on [0, 1], q of degree 8, the relative minimax polynomial from an exchange in double precision (error of u q(u) in
 // float32: 1.7e-7 at most, 5e-8 on average).  As many instructions as the forms above with their two branches, on the FMA pipe.
-__device__ __forceinline__ float2 log1p_unit2(float2 u) {
+__device__ __forceinline__ constexpr float log1p_unit(int i) {
   constexpr float c[] = {0.9999999403953552f, -0.4999949336051941f, 0.3331909775733948f, -0.2484298199415207f, 0.19106006622314453f,
                          -0.13663245737552643f, 0.07822595536708832f, -0.029505237936973572f, 0.0052326940931379795f};
-  float2 q = make_float2(c[8], c[8]);
+  return c[i];
+}
+__device__ __forceinline__ float2 log1p_unit2(float2 u) {
+  float2 q = make_float2(log1p_unit(8), log1p_unit(8));
 #pragma unroll
-  for (int i = 7; i >= 0; --i) q = __ffma2_rn(q, u, make_float2(c[i], c[i]));
+  for (int i = 7; i >= 0; --i) q = __ffma2_rn(q, u, make_float2(log1p_unit(i), log1p_unit(i)));
   return __fmul2_rn(q, u);
 }
 __device__ __forceinline__ float2 softplus_near2(float2 x) {
   const float2 u = make_float2(ex2f(-kLog2e * fabsf(x.x)), ex2f(-kLog2e * fabsf(x.y)));
   return __fadd2_rn(make_float2(fmaxf(x.x, 0.f), fmaxf(x.y, 0.f)), log1p_unit2(u));
 }
-__device__ __forceinline__ float softplus_near(float x) { return softplus_near2(make_float2(x, x)).x; }
+__device__ __forceinline__ float softplus_near(float x) {
+  const float u = ex2f(-kLog2e * fabsf(x));
+  float q = log1p_unit(8);
+#pragma unroll
+  for (int i = 7; i >= 0; --i) q = fmaf(q, u, log1p_unit(i));
+  return fmaf(q, u, fmaxf(x, 0.f));
+}
 // ... and its derivative, the sigmoid, from the same exponential.
 __device__ __forceinline__ float2 softplus_sigmoid_near2(float2 x, float2& sig) {
   const float2 u = make_float2(ex2f(-kLog2e * fabsf(x.x)), ex2f(-kLog2e * fabsf(x.y)));

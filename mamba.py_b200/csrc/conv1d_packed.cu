@@ -36,7 +36,7 @@ __device__ __forceinline__ void load_window(const T* p, Pk<W> (&win)[V / W][kCon
     }
 }
 
-// The thread that meets a sequence's first row also leaves the window: the only one that reads what the slot held.  So the (at most two) rows
+// The thread that meets a sequence's first row also leaves the window, when it is done with its rows: the only one that reads what the slot held.  So the (at most two) rows
 // after a first row that need it too, when they fall into the next chunk, are done by the chunk of the first row.
 template <typename T, int V>
 __global__ void __launch_bounds__(kPkThreads, 3)
@@ -91,38 +91,17 @@ conv1d_silu_packed_fwd_kernel(const Packed seqs, const T* __restrict__ x, const 
 #pragma unroll
     for (int i = 0; i < P; ++i) win[i][k] = xv[i];
   }
-  // What row t, the first of sequence r, enters with; and what the sequence leaves.
-  auto begin = [&](int t, int r) {
+  // What row t, the first of sequence r, enters with.
+  auto begin = [&](int r) {
     const int64_t slot = windows ? seqs.slot(r) : -1;
-    T* const at = windows + (slot * ED + e) * (kConvK - 1);
-    const bool old = slot >= 0 && seqs.resumes(r);
-    if (old) load_window<T, V, W>(at, win);
-    else {
-#pragma unroll
-      for (int i = 0; i < P; ++i)
-#pragma unroll
-        for (int k = 0; k < kConvK - 1; ++k) win[i][k] = F::splat(0.f);
+    if (slot >= 0 && seqs.resumes(r)) {
+      load_window<T, V, W>(windows + (slot * ED + e) * (kConvK - 1), win);
+      return;
     }
-    if (slot < 0) return;
-    const int n = seqs.end(r, t) - t;
-    T v[kConvK - 1][V];
 #pragma unroll
-    for (int k = 0; k < kConvK - 1; ++k) {
-      const int place = n - (kConvK - 1) + k;             // of the input that goes to entry k
-      if (place >= 0) {
-        const CVec<T, V> q = cload<T, V>(x + int64_t(t + place) * x_sl + e, true);
+    for (int i = 0; i < P; ++i)
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[k][i] = q.v[i];
-      } else {                                            // shorter than the window: what was there moves up
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[k][i] = old ? at[3 * i + n + k] : Elem<T>::from_f(0.f);
-      }
-    }
-    CVec<T, V> out[kConvK - 1];
-#pragma unroll
-    for (int j = 0; j < (kConvK - 1) * V; ++j) out[j / V].v[j % V] = v[j % 3][j / 3];
-#pragma unroll
-    for (int k = 0; k < kConvK - 1; ++k) cstore<T, V>(at + k * V, out[k]);
+      for (int k = 0; k < kConvK - 1; ++k) win[i][k] = F::splat(0.f);
   };
   auto group = [&](auto plain, int t) {                   // rows t .. t + 7 below hi; plain: all of them, and no sequence begins
     constexpr bool kPlain = decltype(plain)::value;
@@ -134,7 +113,7 @@ conv1d_silu_packed_fwd_kernel(const Packed seqs, const T* __restrict__ x, const 
     }
 #pragma unroll
     for (int j = 0; j < kPkGroup; ++j) {
-      if (!kPlain && t + j < hi && first_at(t + j)) begin(t + j, mine[t + j - t0 + kBefore] - 1);
+      if (!kPlain && t + j < hi && first_at(t + j)) begin(mine[t + j - t0 + kBefore] - 1);
       F xn[P], o[P];
       unpack<T, V, W>(v[j], xn);
 #pragma unroll
@@ -161,6 +140,37 @@ conv1d_silu_packed_fwd_kernel(const Packed seqs, const T* __restrict__ x, const 
 #pragma unroll
     for (int i = 0; i < V; ++i) zero.v[i] = Elem<T>::from_f(0.f);
     for (int t = max(t0, tail); t < t1; ++t) cstore<T, V>(y + int64_t(t) * y_sl + e, zero);
+    // What the sequences that begin in this chunk leave.
+    if (windows) {
+      for (uint64_t own = firsts >> kBefore & ((uint64_t(1) << kPkChunk) - 1); own; own &= own - 1) {
+        const int t = t0 + __ffsll(int64_t(own)) - 1, r = mine[t - t0 + kBefore] - 1;
+        const int64_t slot = seqs.slot(r);
+        if (slot < 0) continue;
+        T* const at = windows + (slot * ED + e) * (kConvK - 1);
+        const bool old = seqs.resumes(r);
+        const int n = seqs.end(r, t) - t;
+        T v[kConvK - 1][V];
+#pragma unroll
+        for (int k = 0; k < kConvK - 1; ++k) {
+          const int place = n - (kConvK - 1) + k;         // of the input that goes to entry k
+#pragma unroll
+          for (int i = 0; i < V; ++i) v[k][i] = Elem<T>::from_f(0.f);
+          if (place >= 0) {
+            const CVec<T, V> q = cload<T, V>(x + int64_t(t + place) * x_sl + e, true);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[k][i] = q.v[i];
+          } else if (old) {                               // shorter than the window: what was there moves up
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[k][i] = at[3 * i + n + k];
+          }
+        }
+        CVec<T, V> out[kConvK - 1];
+#pragma unroll
+        for (int j = 0; j < (kConvK - 1) * V; ++j) out[j / V].v[j % V] = v[j % 3][j / 3];
+#pragma unroll
+        for (int k = 0; k < kConvK - 1; ++k) cstore<T, V>(at + k * V, out[k]);
+      }
+    }
   }
 }
 
