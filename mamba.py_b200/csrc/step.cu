@@ -56,19 +56,15 @@ ssm_step_kernel(const T* __restrict__ x, const T* __restrict__ delta, const T* _
   const int tid = threadIdx.x;
   const int q = tid % kLPE;
   const int64_t e = int64_t(blockIdx.x) * kEPB + tid / kLPE;
-  const bool ok = e < ED;
   const int64_t b = blockIdx.y, hb = kSlots ? __ldg(slots + b) : b;
-  float yv = 0.f, xv = 0.f;
-  if (kSlots && (hb < 0 || hb >= n_slots)) {
-    if (ok && q == 0) y[b * y_sb + e] = Elem<T>::from_f(0.f);
-    return;
-  }
+  const bool mine = e < ED, ok = mine && (!kSlots || (hb >= 0 && hb < n_slots));
+  float yv = 0.f, xv = 0.f, zv = 0.f;
   if (ok) {
     // the state is the only large stream: get it moving first, everything else is small
     float4 hv[kV];
     const float4* hp = reinterpret_cast<const float4*>(h_in + (hb * ED + e) * N + kSPL * q);
 #pragma unroll
-    for (int v = 0; v < kV; ++v) hv[v] = h_in ? __ldcs(hp + v) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int v = 0; v < kV; ++v) hv[v] = kSlots || h_in ? __ldcs(hp + v) : make_float4(0.f, 0.f, 0.f, 0.f);
     float Av[kSPL];
     if (kF32 || A_.dtype == MB200_F32) {
 #pragma unroll
@@ -101,6 +97,12 @@ ssm_step_kernel(const T* __restrict__ x, const T* __restrict__ delta, const T* _
     }
     xv = Elem<T>::to_f(x[b * x_sb + e]);
     float dv = Elem<T>::to_f(delta[b * d_sb + e]);
+    if constexpr (kSlots) {
+      // Every load is out before the arithmetic begins: the state's wait for the slot's, and what the compiler puts behind them waits for both
+      // (256 rows of 5120 channels on 320 slots 50.4 us without, 36.1 with, 35.0 with the gate's as well; rows in order, no slots: 31.8).
+      if (z) zv = Elem<T>::to_f(z[b * z_sb + e]);
+      asm volatile("" ::: "memory");
+    }
     if (flags & MB200_DELTA_SOFTPLUS) {
       dv += kF32 ? delta_bias[e] : delta_bias_.at(e);
       dv = kSlots ? softplus_near(dv) : softplus_fast(dv);
@@ -127,11 +129,12 @@ ssm_step_kernel(const T* __restrict__ x, const T* __restrict__ delta, const T* _
   if (ok && q == 0) {
     yv = fmaf(D ? (kF32 ? D[e] : D_.at(e)) : 0.f, xv, yv);
     if (z) {
-      const float zv = Elem<T>::to_f(z[b * z_sb + e]);
+      if constexpr (!kSlots) zv = Elem<T>::to_f(z[b * z_sb + e]);
       yv *= zv * sigmoid_fast(zv);
     }
     y[b * y_sb + e] = Elem<T>::from_f(yv);
   }
+  if (kSlots && mine && !ok && q == 0) y[b * y_sb + e] = Elem<T>::from_f(0.f);
 }
 
 // xc = silu(sum_k w[e,k]*win[k] + bias[e]) with win = [conv_in[b,e,:], xin[b,e]]; conv_out = win[1:].
