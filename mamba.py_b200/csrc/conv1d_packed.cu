@@ -13,9 +13,29 @@
 namespace mb200 {
 namespace {
 
-constexpr int kPkThreads = 256, kPkWarps = kPkThreads / 32;
-constexpr int kPkChunk = 32, kPkGroup = 8;
-constexpr int kPkRows = kPkWarps * kPkChunk;           // rows of a forward CTA
+constexpr int kPkThreads = 256, kPkWarps = kPkThreads / 32, kPkResident = 3;
+constexpr int kPkChunk = 32, kPkGroup = 8;              // rows of a forward warp; rows whose loads go out together
+
+// Both sigmoids of a pair from one reciprocal: 1 / (a b) times the other.  The exponentials stay below 2^60 for that (a sigmoid of less is 2^-60).
+// The special function unit, which takes 16 cycles for two results of a warp and was busy for 19 of 42 us at 8000 x 5120, has a quarter less to do.
+__device__ __forceinline__ Pk<1> psigmoid_pk(Pk<1> a) { return psigmoid(a); }
+__device__ __forceinline__ Pk<2> psigmoid_pk(Pk<2> a) {
+  const float2 m = __fmul2_rn(a.v, make_float2(-kLog2e, -kLog2e));
+  const float2 d = __fadd2_rn(make_float2(ex2f(fminf(m.x, 60.f)), ex2f(fminf(m.y, 60.f))), make_float2(1.f, 1.f));
+  const float r = rcpf(d.x * d.y);
+  return {__fmul2_rn(make_float2(r, r), make_float2(d.y, d.x))};
+}
+
+// Where sequences begin: a bit for every row from `base` on.
+struct Firsts {
+  const unsigned* bits;
+  int base;
+  // of 32 rows from t on, lowest first
+  __device__ __forceinline__ unsigned from(int t) const {
+    const int at = t - base;
+    return __funnelshift_r(bits[at >> 5], bits[(at >> 5) + 1], at & 31);
+  }
+};
 
 // Of a pool of windows (n_slots, ED, 3): the windows of V neighbouring channels from e on, oldest input first.
 template <typename T, int V, int W>
@@ -36,86 +56,73 @@ __device__ __forceinline__ void load_window(const T* p, Pk<W> (&win)[V / W][kCon
     }
 }
 
-// The thread that meets a sequence's first row also leaves the window, when it is done with its rows: the only one that reads what the slot held.  So the (at most two) rows
-// after a first row that need it too, when they fall into the next chunk, are done by the chunk of the first row.
+// The thread that meets a sequence's first row also leaves the window, when it is done with its rows: the only one that reads what the slot held.  So
+// the (at most two) rows after a first row that need it too, when they fall into the next chunk, are done by the chunk of the first row.
+// A warp finds out by itself which sequences begin in its rows, a lane a sequence, while the first rows and the filter are on their way: no
+// barrier, and for up to 32 sequences one load.
 template <typename T, int V>
-__global__ void __launch_bounds__(kPkThreads, 3)
+__global__ void __launch_bounds__(kPkThreads, kPkResident)
 conv1d_silu_packed_fwd_kernel(const Packed seqs, const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ bias,
-                              T* __restrict__ y, T* windows, int64_t ED, int64_t x_sl, int64_t y_sl) {
-  constexpr int kBefore = kConvK - 2, kAfter = kConvK - 2;
-  __shared__ int s_first[kBefore + kPkRows + kAfter];     // 1 + the sequence whose first row this is, 0: none's
+                              T* __restrict__ y, T* windows, int64_t ED, int64_t x_sl, int64_t y_sl, int chunks) {
+  constexpr int kG = sizeof(T) * V > 8 ? kPkGroup / 2 : kPkGroup;
+  constexpr int kBefore = kConvK - 2, kSeen = kBefore + kPkChunk + kConvK - 2;
+  struct Begins { int64_t slot; int seq; bool old; };     // a sequence, its slot or -1, and whether it resumes
+  __shared__ Begins s_begins[kPkWarps][kSeen];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int T0 = int(blockIdx.x) * kPkRows;
-  for (int i = threadIdx.x; i < kBefore + kPkRows + kAfter; i += kPkThreads) s_first[i] = 0;
-  __syncthreads();
-  const int tail = seqs.start(seqs.sequences);            // rows from here on belong to no sequence
-  for (int r = threadIdx.x; r < seqs.sequences; r += kPkThreads) {
-    const int first = seqs.start(r);
-    if (seqs.end(r, first) > first && first >= T0 - kBefore && first < T0 + kPkRows + kAfter) s_first[first - T0 + kBefore] = r + 1;
-  }
-  __syncthreads();
-  // bit i: a sequence begins at row t0 - 2 + i
-  constexpr int kSeen = kBefore + kPkChunk + kAfter;
-  static_assert(kSeen > 32 && kSeen <= 64, "two ballots");
-  const int* const mine = s_first + warp * kPkChunk;
-  const uint64_t firsts = uint64_t(__ballot_sync(0xffffffffu, mine[lane] != 0)) |
-                          uint64_t(__ballot_sync(0xffffffffu, lane < kSeen - 32 && mine[lane < kSeen - 32 ? 32 + lane : 0] != 0)) << 32;
+  const int begin = (int(blockIdx.x) * kPkWarps + warp) * kPkChunk * chunks, end = int(min64(int64_t(begin) + kPkChunk * chunks, seqs.rows));
   const int64_t e = (int64_t(blockIdx.y) * 32 + lane) * V;
-  const int t0 = T0 + warp * kPkChunk;
-  if (e >= ED || t0 >= seqs.rows) return;
-  // rows this chunk does: from lo to hi
-  auto first_at = [&](int t) { return t - t0 + kBefore >= 0 && t - t0 + kBefore < kSeen && (firsts >> (t - t0 + kBefore) & 1); };
-  const int t1 = min(t0 + kPkChunk, seqs.rows);
-  int lo = t0, hi = min(t1, tail);
-  // a row within two of its sequence's first one, if that lies in another chunk, belongs to that chunk
-  constexpr int kFar = -2 * kConvK;
-  const int in_front = first_at(t0 - 1) ? t0 - 1 : first_at(t0 - 2) ? t0 - 2 : kFar;
-  const int at_end = t1 != t0 + kPkChunk ? kFar : first_at(t1 - 1) ? t1 - 1 : first_at(t1 - 2) ? t1 - 2 : kFar;
-  while (lo < t1 && lo - in_front < kConvK - 1 && !first_at(lo)) ++lo;
-  while (hi < tail && hi - at_end < kConvK - 1 && !first_at(hi)) ++hi;
+  const bool works = e < ED;
   constexpr int W = (V % 2 == 0) ? 2 : 1, P = V / W;
   using F = Pk<W>;
   F wk[P][kConvK], bv[P], win[P][kConvK - 1];
+  CVec<T, V> front[kConvK - 1], v[kG];
+  Begins* const mine = s_begins[warp];
+  const int tail = seqs.start(seqs.sequences);            // rows from here on belong to no sequence
+  if (works) {
 #pragma unroll
-  for (int i = 0; i < P; ++i) {
-    bv[i] = bias ? F::load(bias + e + W * i, 1) : F::splat(0.f);
+    for (int i = 0; i < P; ++i) {
+      bv[i] = bias ? F::load(bias + e + W * i, 1) : F::splat(0.f);
 #pragma unroll
-    for (int k = 0; k < kConvK; ++k) wk[i][k] = F::load(w + (e + W * i) * kConvK + k, kConvK);
-  }
-  const T* xp = x + int64_t(lo) * x_sl + e;
-  T* yp = y + int64_t(lo) * y_sl + e;
-#pragma unroll
-  for (int k = 0; k < kConvK - 1; ++k) {
-    F xv[P];
-    unpack<T, V, W>(cload<T, V>(xp + (k - (kConvK - 1)) * x_sl, lo + k >= kConvK - 1), xv);
-#pragma unroll
-    for (int i = 0; i < P; ++i) win[i][k] = xv[i];
-  }
-  // What row t, the first of sequence r, enters with.
-  auto begin = [&](int r) {
-    const int64_t slot = windows ? seqs.slot(r) : -1;
-    if (slot >= 0 && seqs.resumes(r)) {
-      load_window<T, V, W>(windows + (slot * ED + e) * (kConvK - 1), win);
-      return;
+      for (int k = 0; k < kConvK; ++k) wk[i][k] = F::load(w + (e + W * i) * kConvK + k, kConvK);
     }
+  }
+#pragma unroll 1
+  for (int t0 = begin; t0 < end; t0 += kPkChunk) {
+    const int t1 = min(t0 + kPkChunk, seqs.rows);
+    const T* xp = x + int64_t(t0) * x_sl + e;
+    if (works) {
 #pragma unroll
-    for (int i = 0; i < P; ++i)
+      for (int k = 0; k < kConvK - 1; ++k) front[k] = cload<T, V>(xp + (k - (kConvK - 1)) * x_sl, t0 + k >= kConvK - 1);
 #pragma unroll
-      for (int k = 0; k < kConvK - 1; ++k) win[i][k] = F::splat(0.f);
-  };
-  auto group = [&](auto plain, int t) {                   // rows t .. t + 7 below hi; plain: all of them, and no sequence begins
-    constexpr bool kPlain = decltype(plain)::value;
-    CVec<T, V> v[kPkGroup];
-#pragma unroll
-    for (int j = 0; j < kPkGroup; ++j) {
-      v[j] = cload<T, V>(xp, kPlain || t + j < hi);
-      xp += x_sl;
+      for (int j = 0; j < kG; ++j) v[j] = cload<T, V>(xp + j * x_sl, t0 + j < t1);
     }
+    // bit i: a sequence begins at row t0 - 2 + i
+    __syncwarp();                                           // (the last chunk's are read)
+    uint64_t firsts = 0;
+    for (int r = lane; r < seqs.sequences; r += 32) {
+      const int first = seqs.start(r), at = first - t0 + kBefore;
+      if (at >= 0 && at < kSeen && seqs.end(r, first) > first) {
+        firsts |= uint64_t(1) << at;
+        mine[at] = Begins{windows ? seqs.slot(r) : -1, r, seqs.resumes(r)};
+      }
+    }
+    __syncwarp();
+    firsts = uint64_t(__reduce_or_sync(0xffffffffu, unsigned(firsts))) | uint64_t(__reduce_or_sync(0xffffffffu, unsigned(firsts >> 32))) << 32;
+    if (!works) continue;
+    T* yp = y + int64_t(t0) * y_sl + e;
+    auto enter = [&]() {
 #pragma unroll
-    for (int j = 0; j < kPkGroup; ++j) {
-      if (!kPlain && t + j < hi && first_at(t + j)) begin(mine[t + j - t0 + kBefore] - 1);
+      for (int k = 0; k < kConvK - 1; ++k) {
+        F xv[P];
+        unpack<T, V, W>(front[k], xv);
+#pragma unroll
+        for (int i = 0; i < P; ++i) win[i][k] = xv[i];
+      }
+    };
+    // y of one row, whose input enters the window
+    auto row = [&](const CVec<T, V>& q) {
       F xn[P], o[P];
-      unpack<T, V, W>(v[j], xn);
+      unpack<T, V, W>(q, xn);
 #pragma unroll
       for (int i = 0; i < P; ++i) {
         F acc = pfma(wk[i][0], win[i][0], bv[i]);
@@ -123,53 +130,108 @@ conv1d_silu_packed_fwd_kernel(const Packed seqs, const T* __restrict__ x, const 
         acc = pfma(wk[i][2], win[i][2], acc);
         acc = pfma(wk[i][3], xn[i], acc);
         win[i][0] = win[i][1]; win[i][1] = win[i][2]; win[i][2] = xn[i];
-        o[i] = pmul(acc, psigmoid(acc));
+        o[i] = pmul(acc, psigmoid_pk(acc));
       }
-      if (kPlain || t + j < hi) cstore<T, V>(yp, pack<T, V, W>(o));
-      yp += y_sl;
-    }
-  };
-  // No sequence begins in the chunk or in the two rows in front of it, and all of it is rows of sequences.
-  if (lo == t0 && hi == t0 + kPkChunk && (firsts & ((uint64_t(1) << (kBefore + kPkChunk)) - 1)) == 0) {
+      return pack<T, V, W>(o);
+    };
+    // No sequence begins in the chunk or in the two rows in front of it, and all of it is rows of sequences.
+    if (t0 + kPkChunk <= tail && (firsts & ((uint64_t(1) << (kBefore + kPkChunk)) - 1)) == 0) {
+      enter();
 #pragma unroll
-    for (int g = 0; g < kPkChunk / kPkGroup; ++g) group(std::true_type{}, t0 + g * kPkGroup);
-  } else {
+      for (int g = 0; g < kPkChunk / kG; ++g) {
+        if (g > 0) {
+#pragma unroll
+          for (int j = 0; j < kG; ++j) v[j] = cload<T, V>(xp + j * x_sl, true);
+        }
+        xp += kG * x_sl;
+#pragma unroll
+        for (int j = 0; j < kG; ++j) {
+          cstore<T, V>(yp, row(v[j]));
+          yp += y_sl;
+        }
+      }
+      continue;
+    }
+    // Rows this chunk does, lo to hi: a row within two of its sequence's first one, if that lies in another chunk, belongs to that chunk.
+    auto first_at = [&](int t) { return (firsts >> (t - t0 + kBefore) & 1) != 0; };
+    int lo = t0, hi = min(t1, tail);
+    constexpr int kFar = -2 * kConvK;
+    const int in_front = first_at(t0 - 1) ? t0 - 1 : first_at(t0 - 2) ? t0 - 2 : kFar;
+    const int at_end = t1 != t0 + kPkChunk ? kFar : first_at(t1 - 1) ? t1 - 1 : first_at(t1 - 2) ? t1 - 2 : kFar;
+    while (lo < t1 && lo - in_front < kConvK - 1 && !first_at(lo)) ++lo;
+    while (hi < tail && hi - at_end < kConvK - 1 && !first_at(hi)) ++hi;
+    xp += int64_t(lo - t0) * x_sl;
+    yp += int64_t(lo - t0) * y_sl;
+    if (lo > t0) {
+#pragma unroll
+      for (int k = 0; k < kConvK - 1; ++k) front[k] = cload<T, V>(xp + (k - (kConvK - 1)) * x_sl, lo + k >= kConvK - 1);
+    }
+    enter();
 #pragma unroll 1
-    for (int t = lo; t < hi; t += kPkGroup) group(std::false_type{}, t);
+    for (int t = lo; t < hi; t += kG) {
+#pragma unroll
+      for (int j = 0; j < kG; ++j) v[j] = cload<T, V>(xp + j * x_sl, t + j < hi);
+      xp += kG * x_sl;
+      if (t + kG <= hi && (firsts >> (t - t0 + kBefore) & ((1u << kG) - 1)) == 0) {
+#pragma unroll
+        for (int j = 0; j < kG; ++j) {
+          cstore<T, V>(yp, row(v[j]));
+          yp += y_sl;
+        }
+        continue;
+      }
+      // (one row at a time, the others moving up: unrolled, what a first row does eight times over costs the path above its registers)
+#pragma unroll 1
+      for (int u = t; u < t + kG && u < hi; ++u) {
+        if (first_at(u)) {
+          const Begins q = mine[u - t0 + kBefore];
+          if (q.slot >= 0 && q.old) {
+            load_window<T, V, W>(windows + (q.slot * ED + e) * (kConvK - 1), win);
+          } else {
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+#pragma unroll
+              for (int k = 0; k < kConvK - 1; ++k) win[i][k] = F::splat(0.f);
+          }
+        }
+        cstore<T, V>(yp, row(v[0]));
+        yp += y_sl;
+#pragma unroll
+        for (int j = 0; j + 1 < kG; ++j) v[j] = v[j + 1];
+      }
+    }
     CVec<T, V> zero;
 #pragma unroll
     for (int i = 0; i < V; ++i) zero.v[i] = Elem<T>::from_f(0.f);
     for (int t = max(t0, tail); t < t1; ++t) cstore<T, V>(y + int64_t(t) * y_sl + e, zero);
+    if (!windows) continue;
     // What the sequences that begin in this chunk leave.
-    if (windows) {
-      for (uint64_t own = firsts >> kBefore & ((uint64_t(1) << kPkChunk) - 1); own; own &= own - 1) {
-        const int t = t0 + __ffsll(int64_t(own)) - 1, r = mine[t - t0 + kBefore] - 1;
-        const int64_t slot = seqs.slot(r);
-        if (slot < 0) continue;
-        T* const at = windows + (slot * ED + e) * (kConvK - 1);
-        const bool old = seqs.resumes(r);
-        const int n = seqs.end(r, t) - t;
-        T v[kConvK - 1][V];
+    for (uint64_t own = firsts >> kBefore & ((uint64_t(1) << kPkChunk) - 1); own; own &= own - 1) {
+      const int t = t0 + __ffsll(int64_t(own)) - 1;
+      const Begins q = mine[t - t0 + kBefore];
+      if (q.slot < 0) continue;
+      T* const at = windows + (q.slot * ED + e) * (kConvK - 1);
+      const int n = seqs.end(q.seq, t) - t;
+      T u[kConvK - 1][V];
 #pragma unroll
-        for (int k = 0; k < kConvK - 1; ++k) {
-          const int place = n - (kConvK - 1) + k;         // of the input that goes to entry k
+      for (int k = 0; k < kConvK - 1; ++k) {
+        const int place = n - (kConvK - 1) + k;             // of the input that goes to entry k
 #pragma unroll
-          for (int i = 0; i < V; ++i) v[k][i] = Elem<T>::from_f(0.f);
-          if (place >= 0) {
-            const CVec<T, V> q = cload<T, V>(x + int64_t(t + place) * x_sl + e, true);
+        for (int i = 0; i < V; ++i) u[k][i] = Elem<T>::from_f(0.f);
+        if (place >= 0) {
+          const CVec<T, V> in = cload<T, V>(x + int64_t(t + place) * x_sl + e, true);
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[k][i] = q.v[i];
-          } else if (old) {                               // shorter than the window: what was there moves up
+          for (int i = 0; i < V; ++i) u[k][i] = in.v[i];
+        } else if (q.old) {                                 // shorter than the window: what was there moves up
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[k][i] = at[3 * i + n + k];
-          }
+          for (int i = 0; i < V; ++i) u[k][i] = at[3 * i + n + k];
         }
-        CVec<T, V> out[kConvK - 1];
-#pragma unroll
-        for (int j = 0; j < (kConvK - 1) * V; ++j) out[j / V].v[j % V] = v[j % 3][j / 3];
-#pragma unroll
-        for (int k = 0; k < kConvK - 1; ++k) cstore<T, V>(at + k * V, out[k]);
       }
+      CVec<T, V> out[kConvK - 1];
+#pragma unroll
+      for (int j = 0; j < (kConvK - 1) * V; ++j) out[j / V].v[j % V] = u[j % 3][j / 3];
+#pragma unroll
+      for (int k = 0; k < kConvK - 1; ++k) cstore<T, V>(at + k * V, out[k]);
     }
   }
 }
@@ -177,7 +239,7 @@ conv1d_silu_packed_fwd_kernel(const Packed seqs, const T* __restrict__ x, const 
 // dx[t] = sum_j w[3-j] * dpre[t+j] over the rows t+j of t's sequence;  dw[k] = sum_t dpre[t] * in(t-3+k);  dbias = sum dpre;
 // dpre[t] = dy[t] * silu'(pre[t]), pre recomputed from x.  Sequences that resume have no backward, so in = 0 before a first row.
 // As on rectangles the windows hold as many rows as a group, dx trails by three rows, and the 4 warps of a CTA add their sums in shared memory.
-constexpr int kPkBwdThreads = 128, kPkBwdWarps = kPkBwdThreads / 32, kPkBwdChunkMost = 64;
+constexpr int kPkBwdThreads = 128, kPkBwdWarps = kPkBwdThreads / 32, kPkBwdChunkMost = 128;
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kPkBwdThreads, 4)
@@ -220,11 +282,8 @@ conv1d_silu_packed_bwd_kernel(const Packed seqs, const T* __restrict__ x, const 
 #pragma unroll
       for (int k = 0; k < kG; ++k) dw_[i][k] = F::splat(0.f);
     }
-    // bits of rows t - 3 .. t + 3, lowest first
-    auto firsts_at = [&](int t) {
-      const int at = t - T0;
-      return __funnelshift_r(s_first[at >> 5], s_first[(at >> 5) + 1], at & 31) & 0x7fu;
-    };
+    const Firsts firsts{s_first, T0 - kH};
+    auto firsts_at = [&](int t) { return firsts.from(t - kH) & 0x7fu; };       // of rows t - 3 .. t + 3
     const T* xg = x + int64_t(t0) * x_sl + e;
     const T* gg = dy + int64_t(t0) * dy_sl + e;
     T* og = dx + int64_t(t0 - kH) * dx_sl + e;
@@ -267,7 +326,7 @@ conv1d_silu_packed_bwd_kernel(const Packed seqs, const T* __restrict__ x, const 
           F pre = bv[i];
 #pragma unroll
           for (int k = 0; k < kConvK; ++k) pre = pfma(wk[i][k], xw[i][(j + 1 + k) % kG], pre);
-          const F sg = psigmoid(pre);
+          const F sg = psigmoid_pk(pre);
           const F dp = pmul(pmul(g[i], sg), pfma(pre, pfma(sg, mone, one), one));
           dw_[i][j] = dp;
           // dx[t-3] = w3*dpre[t-3] + w2*dpre[t-2] + w1*dpre[t-1] + w0*dpre[t]
@@ -319,6 +378,19 @@ conv1d_silu_packed_bwd_kernel(const Packed seqs, const T* __restrict__ x, const 
   }
 }
 
+// Rows of a warp, a multiple of `unit`: as many as make the rounds of CTAs that fit the SMs, and what each round costs besides its rows (`extra` rows'
+// worth: the way of the first loads, the filter, where sequences begin, the rows in front), cheapest.
+int packed_chunk(int64_t rows, int64_t cols, int warps, int resident, int unit, int most, int extra) {
+  int best = unit;
+  int64_t best_cost = int64_t(1) << 62;
+  for (int c = unit; c <= most; c += unit) {
+    const int64_t ctas = cols * ((rows + warps * c - 1) / (warps * c)), fit = int64_t(sm_count()) * resident;
+    const int64_t cost = (ctas + fit - 1) / fit * (c + extra);
+    if (cost < best_cost) { best_cost = cost; best = c; }
+  }
+  return best;
+}
+
 int check_conv(const mb200_packed* seqs, int64_t ED, int K, int dtype) {
   if (const int rc = packed_check(seqs)) return rc;
   if (ED < 0) return MB200_EINVAL;
@@ -340,10 +412,12 @@ extern "C" int mb200_conv1d_silu_packed_fwd(const mb200_packed* seqs, const void
   const int kv = 4;
   const bool vec = conv_vec_ok(ED, kv, {x, y, (const void*)windows}, {x_sl, y_sl});
   const int v = vec ? kv : 1;
-  const dim3 grid(unsigned((seqs->rows + kPkRows - 1) / kPkRows), unsigned((ED + 32 * int64_t(v) - 1) / (32 * int64_t(v))));
+  const int64_t cols = (ED + 32 * int64_t(v) - 1) / (32 * int64_t(v));
+  const int chunks = packed_chunk(seqs->rows, cols, kPkWarps, kPkResident, kPkChunk, 16 * kPkChunk, 16) / kPkChunk;
+  const dim3 grid(unsigned((seqs->rows + kPkWarps * kPkChunk * chunks - 1) / (kPkWarps * kPkChunk * chunks)), unsigned(cols));
   const Packed k = packed_of(*seqs, 0);
   if (!seqs->slots) windows = nullptr;
-#define MB200_CONV_FWD(TT, VV) conv1d_silu_packed_fwd_kernel<TT, VV><<<grid, kPkThreads, 0, st>>>(k, (const TT*)x, w, bias, (TT*)y, (TT*)windows, ED, x_sl, y_sl)
+#define MB200_CONV_FWD(TT, VV) conv1d_silu_packed_fwd_kernel<TT, VV><<<grid, kPkThreads, 0, st>>>(k, (const TT*)x, w, bias, (TT*)y, (TT*)windows, ED, x_sl, y_sl, chunks)
   if (dtype == MB200_F32) { if (vec) MB200_CONV_FWD(float, 4); else MB200_CONV_FWD(float, 1); }
   else { if (vec) MB200_CONV_FWD(__nv_bfloat16, 4); else MB200_CONV_FWD(__nv_bfloat16, 1); }
 #undef MB200_CONV_FWD
@@ -360,8 +434,9 @@ extern "C" int mb200_conv1d_silu_packed_bwd(const mb200_packed* seqs, const void
   const int kv = 4;
   const bool vec = conv_vec_ok(ED, kv, {x, dy, (const void*)dx}, {x_sl, dy_sl, dx_sl});
   const int v = vec ? kv : 1;
-  const int chunk = 32;
-  const dim3 grid(unsigned((seqs->rows + kPkBwdWarps * chunk - 1) / (kPkBwdWarps * chunk)), unsigned((ED + 32 * int64_t(v) - 1) / (32 * int64_t(v))));
+  const int64_t cols = (ED + 32 * int64_t(v) - 1) / (32 * int64_t(v));
+  const int chunk = packed_chunk(seqs->rows, cols, kPkBwdWarps, 4, 8, kPkBwdChunkMost, 16);
+  const dim3 grid(unsigned((seqs->rows + kPkBwdWarps * chunk - 1) / (kPkBwdWarps * chunk)), unsigned(cols));
   const Packed k = packed_of(*seqs, 0);
 #define MB200_CONV_BWD(TT, VV) \
   conv1d_silu_packed_bwd_kernel<TT, VV><<<grid, kPkBwdThreads, 0, st>>>(k, (const TT*)x, w, bias, (const TT*)dy, (TT*)dx, dw, dbias, ED, x_sl, dy_sl, dx_sl, chunk)
