@@ -12,17 +12,21 @@ namespace {
 // nothing above -inf, has none: what is no candidate counts as -inf, and still fills up places that are left, lowest first.
 //
 // The order is that of the values in 64 bits, at the price of 32: the logsumexp is off by a few 2^-20 (see too_close), and where candidates of
-// different beams come that close, which is a few groups in a hundred calls, the joining CTA sums the group's exponentials again in 64 bits.
+// different beams come that close, which is a few groups in a hundred calls, the joining CTA sums those beams' exponentials again in 64 bits.
 
-constexpr int kSelThreads = 256, kSelWarps = kSelThreads / 32, kSelPer = 32;             // logits of a thread
-constexpr int kSelSlice = kSelThreads * kSelPer;
+constexpr int kSelThreads = 256, kSelWarps = kSelThreads / 32, kSelPer = 16;             // logits of a thread at a time
+constexpr int kSelChunk = kSelThreads * kSelPer;
 constexpr int kMostNum = 64, kMostBeams = 64;
-constexpr int kList = 1024, kJoinList = 512;               // items side by side in shared memory
+constexpr int kList = 1024;                                // items side by side in shared memory
+constexpr int kCheck = 4;                                  // chunks after which the list is looked at
 
 // By how much two logsumexps may be apart for rounding alone.  An exponent t = (v - top) log2(e) is off by 2.25 x 2^-24 |t| (a difference, a product,
-// a constant), and the mean of |t| under the softmax is at most log2 of the vocabulary; ex2.approx is off by 2^-22 of its value; a thread
-// adds 8 terms four times and those, and the threads' sums are added in 64 bits.  In units of 2^-24 of the sum, twice:
-__device__ __forceinline__ double too_close(int V) { return 2 * 0x1p-24 * (2.25 * 0.6931472 * log2(double(V)) + 4. + 10.); }
+// a constant), and the mean of |t| under the softmax is at most log2 of the vocabulary; it goes to the thread's maximum, from there to the CTA's and
+// to the beam's, 3 steps that share |t|, with an ex2.approx of 2^-22 each (a new maximum of the thread is one more, at worst once a chunk, of which all
+// but the last then count for little); a thread adds 16 logits in fours; all further sums are in 64 bits.  In units of 2^-24, twice:
+__device__ __forceinline__ double too_close(int V) {
+  return 2 * 0x1p-24 * (2.25 * 0.6931472 * log2(double(V)) + 4. * 4 + 5.);
+}
 
 // Unsigned order of floats, and of doubles.
 __device__ __forceinline__ uint32_t order_of(float v) {
@@ -48,155 +52,240 @@ struct Slice {
 };
 
 __device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
-__device__ __forceinline__ uint64_t min64u(uint64_t a, uint64_t b) { return a < b ? a : b; }
 
-// The num-th highest of the lanes' keys (num <= 32): the lanes sort them.
-__device__ __forceinline__ uint64_t nth_of_warp(uint64_t key, int num, int lane) {
+// The lanes' values in falling order.
+__device__ __forceinline__ uint32_t sorted_in_warp(uint32_t x, int lane) {
 #pragma unroll
   for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
     for (int step = size / 2; step >= 1; step >>= 1) {
-      const uint64_t other = __shfl_xor_sync(0xffffffffu, key, step);
-      const bool lower = (lane & step) == 0, falling = (lane & size) == 0;
-      key = lower == falling ? max64(key, other) : min64u(key, other);
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, x, step);
+      x = ((lane & step) == 0) == ((lane & size) == 0) ? max(x, other) : min(x, other);
     }
-  return __shfl_sync(0xffffffffu, key, num - 1);
+  return x;
 }
 
-// How the highest are found.  A warp in which num lanes hold a key as high as K holds num that high, so no key below K is wanted; K is the num-th
-// highest of the lanes' own highest, and the CTA takes the highest K of its warps.  What reaches it (a few more than num in general) is put
-// side by side and every item counts those ahead of it.  With more than 32 wanted the halves of a lane's logits stand for lanes, and K is
-// the lowest of their 64.  Where more reach K than there is room for, num rounds of a maximum over the CTA find them.
-// Bound: 8 instructions a logit (load and conversion, maximum, exponent, ex2, sum, two for the place of the maximum, one comparison with K), which
-// is near the time that its 2 bytes take from HBM; three CTAs on an SM cover each other's barriers.
+// How the highest are found.  A warp in which num lanes hold a value as high as K holds num that high, and so do the kSelWarps warps together if
+// each has its share of lanes that high; so no logit below K is wanted.  The higher of the two, over the slice's first chunk and the threads' own
+// highest, is K.  Whatever reaches K, in the chunks that follow too (about num a chunk, if they are alike), is put side by side with its place, and
+// every item counts those ahead of it; between chunks the num-th of them becomes the new K.  That may be a
+// value that very many logits share (a mask's): equal to K, then, counts only up to the num-th place that does, of which there are num in the
+// first chunk or none.  Should a chunk have more than there is room for all the same (ascending logits may), num rounds over the slice find the highest.
+// Bound: 8 instructions a logit (load and conversion, maximum, difference, product, ex2, sum), which is near the time that its 2 bytes take
+// from HBM, and some 2 us a CTA for the first chunk's sort and the counts at the end.  So a CTA takes as many chunks as leave
+// four CTAs for every SM, with the next chunk's loads in flight.  64 x 4 x 50280 in bfloat16: 58 us with a CTA to every 8192 logits and a count of
+// all threads' highest, 25 with the warps' sort, 22 with several chunks a CTA.
 template <typename T, bool kVec>
-__global__ void __launch_bounds__(kSelThreads, 3)
-beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int num, Slice* __restrict__ slices, uint64_t* __restrict__ best) {
-  __shared__ uint64_t s_list[kList], s_least[kSelWarps];
+__global__ void __launch_bounds__(kSelThreads, 4)
+beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slice, int num, Slice* __restrict__ slices, uint64_t* __restrict__ best) {
+  __shared__ uint64_t s_list[kList], s_best[kMostNum], s_key[kSelWarps];
+  __shared__ uint32_t s_least[2][kSelWarps];
   __shared__ float s_top[kSelWarps];
   __shared__ double s_sum[kSelWarps];
   __shared__ int s_n;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = blockIdx.y, part = row * gridDim.x + blockIdx.x;
-  const int v0 = int(blockIdx.x) * kSelSlice;
+  const int v0 = int(blockIdx.x) * slice, v1 = min(V, v0 + slice);
   const T* p = logits + row * stride;
   if (tid == 0) s_n = 0;
   cudaTriggerProgrammaticLaunchCompletion();               // the joining kernel may start, and waits for this one's end
   constexpr int kE = kVec ? Elem<T>::kVec : 1, kLoads = kSelPer / kE;
-  float v[kSelPer];
-  auto at = [&](int j) { return v0 + ((j / kE) * kSelThreads + tid) * kE + j % kE; };
+  struct alignas(sizeof(T) * kE) Raw { T v[kE]; };
+  auto at = [&](int c0, int j) { return c0 + ((j / kE) * kSelThreads + tid) * kE + j % kE; };
+  auto fetch = [&](int c0, Raw (&raw)[kLoads]) {
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int c = at(i * kE);
-    if (kVec && c + kE <= V) {
-      if constexpr (kVec) {
-        const Vec16<T> q = ldcs16(p + c);
+    for (int i = 0; i < kLoads; ++i) {
+      const int c = at(c0, i * kE);
+      if (kVec && c + kE <= v1) {
+        if constexpr (kVec) *reinterpret_cast<uint4*>(&raw[i]) = __ldcs(reinterpret_cast<const uint4*>(p + c));
+      } else {
 #pragma unroll
-        for (int k = 0; k < kE; ++k) v[i * kE + k] = Elem<T>::to_f(q.v[k]);
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < kE; ++k) v[i * kE + k] = c + k < V ? Elem<T>::to_f(p[c + k]) : -INFINITY;
-    }
-  }
-  // the highest of each half of the thread's logits, and where
-  float high[2] = {-INFINITY, -INFINITY};
-  int place[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int j = 0; j < kSelPer / 2; ++j) high[h] = fmaxf(high[h], v[h * kSelPer / 2 + j]);
-    place[h] = at(h * kSelPer / 2);
-#pragma unroll
-    for (int j = kSelPer / 2 - 1; j >= 0; --j)
-      if (v[h * kSelPer / 2 + j] == high[h]) place[h] = at(h * kSelPer / 2 + j);
-  }
-  float top = fmaxf(high[0], high[1]);
-  const uint64_t key0 = key_of(high[0], place[0]), key1 = key_of(high[1], place[1]);
-  uint64_t least;
-  if (num <= 32) {
-    least = nth_of_warp(max64(key0, key1), num, lane);
-  } else {
-    least = min64u(key0, key1);
-#pragma unroll
-    for (int s = 16; s >= 1; s >>= 1) least = min64u(least, __shfl_xor_sync(0xffffffffu, least, s));
-  }
-#pragma unroll
-  for (int s = 16; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-  if (lane == 0) {
-    s_top[warp] = top;
-    s_least[warp] = least;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kSelWarps; ++w) {
-    top = fmaxf(top, s_top[w]);
-    least = max64(least, s_least[w]);
-  }
-  const float least_v = value_of(uint32_t(least >> 32));
-  float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int j = 0; j < kSelPer; ++j) {
-    sum4[j % 4] += ex2f((v[j] - top) * kLog2e);
-    if (v[j] >= least_v) {
-      const uint64_t key = key_of(v[j], at(j));
-      if (key >= least && at(j) < V) {
-        const int n = atomicAdd(&s_n, 1);
-        if (n < kList) s_list[n] = key;
+        for (int k = 0; k < kE; ++k) raw[i].v[k] = c + k < v1 ? p[c + k] : Elem<T>::from_f(-INFINITY);
       }
     }
-  }
-  if (top == -INFINITY) {                                  // -inf - -inf: nothing to sum, unless there is a NaN
-    sum4[0] = sum4[1] = sum4[2] = sum4[3] = 0.f;
-#pragma unroll
-    for (int j = 0; j < kSelPer; ++j)
-      if (v[j] != v[j]) sum4[0] = v[j];
-  }
-  double all = (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
-#pragma unroll
-  for (int s = 16; s >= 1; s >>= 1) all += __shfl_xor_sync(0xffffffffu, all, s);
-  if (lane == 0) s_sum[warp] = all;
-  __syncthreads();
-  if (tid == 0) {
-    all = 0.;
-    for (int w = 0; w < kSelWarps; ++w) all += s_sum[w];
-    slices[part] = Slice{top, 0.f, all};
-  }
-  const int n = s_n;
-  uint64_t* const out = best + part * num;
-  if (n <= kList) {
+  };
+  // num highest of the list, highest first, in s_best
+  auto rank = [&](int n) {
     for (int i = tid; i < n; i += kSelThreads) {
       const uint64_t key = s_list[i];
       int ahead = 0;
 #pragma unroll 4
       for (int k = 0; k < n; ++k) ahead += s_list[k] > key;
-      if (ahead < num) out[ahead] = key;
+      if (ahead < num) s_best[ahead] = key;
     }
-    for (int i = n + tid; i < num; i += kSelThreads) out[i] = 0;
-    return;
-  }
-  uint64_t last = ~uint64_t(0);
-  for (int r = 0; r < num; ++r) {
-    uint64_t key = 0;
+    __syncthreads();
+  };
+  Raw raw[kLoads];
+  fetch(v0, raw);
+  float least = -INFINITY;                                 // K
+  int within = v1;                                         // equal to K counts below this place
+  float mine = -INFINITY;                                  // the thread's maximum,
+  double all = 0.;                                         // and its sum of exp(logit - maximum)
+  bool room = true;
+  for (int c0 = v0, chunk = 0; c0 < v1; c0 += kSelChunk, ++chunk) {
+    float v[kSelPer];
+#pragma unroll
+    for (int j = 0; j < kSelPer; j += 2) {
+      if constexpr (kVec) {
+        const float2 two = pair_f(&raw[j / kE].v[j % kE]);
+        v[j] = two.x; v[j + 1] = two.y;
+      } else {
+        v[j] = Elem<T>::to_f(raw[j].v[0]); v[j + 1] = Elem<T>::to_f(raw[j + 1].v[0]);
+      }
+    }
+    if (c0 + kSelChunk < v1) fetch(c0 + kSelChunk, raw);
+    float high = -INFINITY, high2 = -INFINITY;             // of the halves
+#pragma unroll
+    for (int j = 0; j < kSelPer / 2; ++j) {
+      high = fmaxf(high, v[j]);
+      high2 = fmaxf(high2, v[kSelPer / 2 + j]);
+    }
+    if (chunk == 0) {
+      // (with more than 32 wanted, the halves' lowest stands for 64 lanes)
+      const uint32_t x = sorted_in_warp(order_of(fmaxf(high, high2)), lane);
+      uint32_t whole = __shfl_sync(0xffffffffu, x, (num <= 32 ? num : 32) - 1);
+      if (num > 32) whole = __reduce_min_sync(0xffffffffu, order_of(fminf(high, high2)));
+      const uint32_t share = __shfl_sync(0xffffffffu, x, (num + kSelWarps - 1) / kSelWarps - 1);
+      if (lane == 0) {
+        s_least[0][warp] = whole;
+        s_least[1][warp] = share;
+      }
+      __syncthreads();
+      uint32_t most = 0, all = ~0u;
+#pragma unroll
+      for (int w = 0; w < kSelWarps; ++w) {
+        most = max(most, s_least[0][w]);
+        all = min(all, s_least[1][w]);
+      }
+      least = value_of(max(most, all));
+      // The usual number of logits this high is little more than num.  If many are equal to K, the num-th place that is closes it for the others.
+      int equal = 0;
+#pragma unroll
+      for (int j = 0; j < kSelPer; ++j) equal += v[j] == least && at(c0, j) < v1;
+      if (__syncthreads_or(equal > 2)) {
+        // places are in the order of load, thread and element: counted load by load
+        int before = 0;
+        for (int i = 0; i < kLoads; ++i) {
+          int n = 0;
+#pragma unroll
+          for (int j = 0; j < kSelPer; ++j) n += j / kE == i && v[j] == least && at(c0, j) < v1;
+          int upto = n;
+#pragma unroll
+          for (int s = 1; s < 32; s <<= 1) {
+            const int more = __shfl_up_sync(0xffffffffu, upto, s);
+            if (lane >= s) upto += more;
+          }
+          __syncthreads();
+          if (lane == 31) s_least[0][warp] = upto;
+          __syncthreads();
+          int total = 0;
+          for (int w = 0; w < kSelWarps; ++w) {
+            if (w < warp) upto += s_least[0][w];
+            total += s_least[0][w];
+          }
+          int rank_of = before + upto - n;
+#pragma unroll
+          for (int j = 0; j < kSelPer; ++j)
+            if (j / kE == i && v[j] == least && at(c0, j) < v1 && rank_of++ == num - 1) s_n = -at(c0, j) - 1;
+          before += total;
+        }
+        __syncthreads();
+        if (s_n < 0) within = -s_n;                        // behind the num-th such place
+        __syncthreads();
+        if (tid == 0) s_n = 0;
+        __syncthreads();
+      }
+    }
+    const float top = fmaxf(mine, fmaxf(high, high2));
+    if (top > mine) {
+      all *= double(ex2f((mine - top) * kLog2e));          // (0 from -inf)
+      mine = top;
+    }
+    const float from = top == -INFINITY ? 0.f : top;
+    float sum4[4];
 #pragma unroll
     for (int j = 0; j < kSelPer; ++j) {
-      const uint64_t k = key_of(v[j], at(j));
-      if (at(j) < V && k < last) key = max64(key, k);
+      const float x = ex2f((v[j] - from) * kLog2e);
+      sum4[j % 4] = j < 4 ? x : sum4[j % 4] + x;
     }
+    all += double((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+    // Few threads look at their logits one by one, and read those that count again: a body for each of the 16 would cost more than all the rest.
+    if (fmaxf(high, high2) >= least) {
+      unsigned hits = 0;
 #pragma unroll
-    for (int s = 16; s >= 1; s >>= 1) key = max64(key, __shfl_xor_sync(0xffffffffu, key, s));
+      for (int j = 0; j < kSelPer; ++j) hits |= unsigned(v[j] >= least) << j;
+#pragma unroll 1
+      for (; hits; hits &= hits - 1) {
+        const int c = at(c0, __ffs(int(hits)) - 1);
+        const float x = c < v1 ? Elem<T>::to_f(p[c]) : -INFINITY;
+        if (c >= (x == least ? within : v1)) continue;
+        const int n = atomicAdd(&s_n, 1);
+        if (n < kList) s_list[n] = key_of(x, c);
+      }
+    }
+    if (c0 + kSelChunk >= v1) break;
+    if (chunk % kCheck != 0) continue;
     __syncthreads();
-    if (lane == 0) s_least[warp] = key;
+    const int n = s_n;
+    if (n > kList) {
+      room = false;
+    } else if (n > 2 * num && room) {
+      rank(n);
+      if (tid < num) s_list[tid] = s_best[tid];
+      if (tid == 0) s_n = num;
+      // places only rise from here on, so nothing equal to the num-th of these is wanted any more
+      least = value_of(uint32_t(s_best[num - 1] >> 32));
+      within = 0;
+    }
     __syncthreads();
+  }
+  float top = mine;
 #pragma unroll
-    for (int w = 0; w < kSelWarps; ++w) key = max64(key, s_least[w]);
-    if (tid == 0) out[r] = key;
-    last = key;
+  for (int s = 16; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+  if (lane == 0) s_top[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) top = fmaxf(top, s_top[w]);
+  if (top > -INFINITY) all *= double(ex2f((mine - top) * kLog2e));
+#pragma unroll
+  for (int s = 16; s >= 1; s >>= 1) all += __shfl_xor_sync(0xffffffffu, all, s);
+  if (lane == 0) s_sum[warp] = all;
+  const int n = s_n;
+  uint64_t* const out = best + part * num;
+  if (room && n <= kList) {
+    rank(n);
+    for (int i = tid; i < num; i += kSelThreads) out[i] = i < n ? s_best[i] : 0;
+  } else {
+    uint64_t last = ~uint64_t(0);
+    for (int r = 0; r < num; ++r) {
+      uint64_t key = 0;
+      for (int c = v0 + tid; c < v1; c += kSelThreads) {
+        const uint64_t k = key_of(Elem<T>::to_f(p[c]), c);
+        if (k < last) key = max64(key, k);
+      }
+#pragma unroll
+      for (int s = 16; s >= 1; s >>= 1) key = max64(key, __shfl_xor_sync(0xffffffffu, key, s));
+      __syncthreads();
+      if (lane == 0) s_key[warp] = key;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kSelWarps; ++w) key = max64(key, s_key[w]);
+      if (tid == 0) out[r] = key;
+      last = key;
+    }
+  }
+  if (tid == 0) {
+    all = 0.;
+    for (int w = 0; w < kSelWarps; ++w) all += s_sum[w];
+    slices[part] = Slice{top, 0.f, all};
   }
 }
 
-// One CTA a group.  Candidates are looked at kSelThreads at a time; those ahead of the num-th highest so far go side by side in shared
-// memory, and when there are many, and at the end, each counts those ahead of it.
+// One CTA a group.  Every slice lists its highest in falling order, so candidates are taken by their rank in the lists, all lists' first ones first, as many
+// ranks at a time as the threads can take; once a whole rank holds nothing ahead of the num-th highest so far, no further one does.  What
+// the argument above on lanes and warps does not rule out goes side by side in shared memory, where each counts those ahead of it.
+// Bound by latency: two round trips to global memory, a logarithm in 64 bits, and three or four barriers for every set of ranks (one or two sets in
+// general).  16 groups of 16 beams of 128256, 32 of them: 61 us with all 1024 candidates of a group in any order.
 __global__ void __launch_bounds__(kSelThreads)
 beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ best, const float* __restrict__ scores,
                  const uint8_t* __restrict__ finished, const void* __restrict__ logits, int64_t stride, int dtype, int beams, int n_slices, int V,
@@ -205,126 +294,153 @@ beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ 
   __shared__ float s_score[kMostBeams], s_top[kMostBeams];
   __shared__ uint8_t s_kind[kMostBeams];
   __shared__ double s_sum[kSelWarps];
-  // an item: the value's order in 64 bits, and beam * V + token
-  __shared__ uint64_t s_order[kJoinList + kMostNum];
-  __shared__ uint64_t s_flat[kJoinList + kMostNum];
-  __shared__ uint64_t s_best[2][kMostNum];
+  // an item: the value's order in 64 bits, and beam << 32 | token
+  __shared__ uint64_t s_order[kSelThreads + kMostNum], s_place[kSelThreads + kMostNum], s_best[2][kMostNum];
+  __shared__ uint32_t s_least[2][kSelWarps], s_close[kMostBeams / 32];       // beams that are too close to one another
   __shared__ int s_n;
   enum { kOpen, kFinished, kDead };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t g = blockIdx.x;
+  // Lists of the group, and how a set of candidates is made of them: whole ranks of all lists, or a part of one.
+  const int lists = beams * n_slices, ranks = lists <= kSelThreads ? kSelThreads / lists : 1, parts = (lists + kSelThreads - 1) / kSelThreads;
+  const int sets = parts > 1 ? num * parts : (num + ranks - 1) / ranks;
+  auto list_of = [&](int set) { return parts > 1 ? set % parts * kSelThreads + tid : tid < ranks * lists ? tid % lists : lists; };
+  auto rank_of = [&](int set) { return parts > 1 ? set / parts : set * ranks + tid / lists; };
+  const uint64_t* const mine = best + g * lists * num;
+  auto fetch = [&](int set) -> uint64_t {
+    const int l = list_of(set), r = rank_of(set);
+    return l < lists && r < num ? mine[int64_t(l) * num + r] : 0;
+  };
   cudaGridDependencySynchronize();
+  const uint64_t first_key = fetch(0);
   for (int k = warp; k < beams; k += kSelWarps) {          // a warp a beam
     const int64_t row = g * beams + k;
     const Slice* const part = slices + row * n_slices;
+    Slice one{-INFINITY, 0.f, 0.};
+    if (lane < n_slices) one = part[lane];
     const float score = scores[row];
-    int kind = kFinished;
-    double total = 0.;
-    float top = -INFINITY;
-    if (!(finished && finished[row])) {
-      for (int i = lane; i < n_slices; i += 32) top = fmaxf(top, part[i].top);
+    const bool done = finished && finished[row];
+    float top = one.top;
+    for (int i = lane + 32; i < n_slices; i += 32) top = fmaxf(top, part[i].top);
 #pragma unroll
-      for (int s = 16; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-      double sum = 0.;
-      for (int i = lane; i < n_slices; i += 32) sum += part[i].sum * exp(double(part[i].top) - double(top));
+    for (int s = 16; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    double sum = one.sum * double(ex2f((one.top - top) * kLog2e));
+    for (int i = lane + 32; i < n_slices; i += 32) sum += part[i].sum * double(ex2f((part[i].top - top) * kLog2e));
 #pragma unroll
-      for (int s = 16; s >= 1; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-      kind = isfinite(top) && isfinite(sum) ? kOpen : kDead;
-      if (kind == kOpen) total = log(sum);
-    }
+    for (int s = 16; s >= 1; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
     if (lane == 0) {
-      s_total[k] = total;
+      s_total[k] = log(sum);
       s_score[k] = score;
       s_top[k] = top;
-      s_kind[k] = uint8_t(isfinite(score) ? kind : kDead);
+      s_kind[k] = uint8_t(!isfinite(score) ? kDead : done ? kFinished : isfinite(top) && isfinite(sum) ? kOpen : kDead);
     }
   }
+  if (tid == 0) s_n = 0;
+  if (tid < kMostBeams / 32) s_close[tid] = 0;
   __syncthreads();
-  // Candidate i of the group: order (0: none) and place.  What is no candidate stands in at -inf, lowest tokens first: of those, a slice lists enough
-  // among its highest logits if it has fewer than num others, and if one has not, no stand-in is needed.
-  const int each = n_slices * num, all = beams * each;
+  // The thread's candidate of a set: order (0: none) and place.  What is no candidate stands in at -inf, lowest tokens first: of those, a slice lists
+  // enough among its highest logits if it has fewer than num others, and if one has not, no stand-in is needed.
   const uint64_t nothing = order_of(-double(INFINITY));
-  auto candidate = [&](int i, uint64_t& flat) -> uint64_t {
-    const int k = i / each, j = i - k * each, kind = s_kind[k];
-    flat = uint64_t(k) * uint64_t(V);
+  auto candidate = [&](int set, uint64_t& place) -> uint64_t {
+    const int l = list_of(set), r = rank_of(set);
+    if (l >= lists || r >= num) return 0;
+    const int k = l / n_slices, kind = s_kind[k];
+    place = uint64_t(k) << 32;
     if (kind == kOpen) {
-      const uint64_t key = best[g * all + i];
-      flat += uint32_t(~uint32_t(key));
+      const uint64_t key = set == 0 ? first_key : mine[int64_t(l) * num + r];
+      place |= uint32_t(~uint32_t(key));
       return key ? order_of(double(s_score[k]) + ((double(value_of(uint32_t(key >> 32))) - double(s_top[k])) - s_total[k])) : 0;
     }
-    if (kind == kFinished && j == 0) {
-      flat += end_token;
-      return order_of(double(s_score[k]));
+    if (l != k * n_slices) return 0;                       // the first slice's list stands for such a beam
+    int t = r;
+    if (kind == kFinished) {
+      if (r == 0) {
+        place |= uint32_t(end_token);
+        return order_of(double(s_score[k]));
+      }
+      if (--t >= end_token) ++t;
     }
-    int t = kind == kFinished ? j - 1 : j;
-    if (kind == kFinished && t >= end_token) ++t;
-    flat += t;
-    return t < V && j < num ? nothing : 0;
+    place |= uint32_t(t);
+    return t < V ? nothing : 0;
   };
   for (bool again = false;; again = true) {
-    uint64_t least_order = 0, least_flat = 0;              // of the num-th highest so far
-    if (tid == 0) s_n = 0;
-    __syncthreads();
-    for (int base = 0; base < all; base += kSelThreads) {
-      if (base + tid < all) {
-        uint64_t flat;
-        const uint64_t order = candidate(base + tid, flat);
-        if (order && (order > least_order || (order == least_order && flat < least_flat))) {
-          const int n = atomicAdd(&s_n, 1);
-          s_order[n] = order;
-          s_flat[n] = flat;
-        }
+    uint64_t least_order = 0, least_place = 0;             // of the num-th highest so far
+    bool fresh = false;                                    // something of this rank went into the list
+    for (int set = 0; set < sets; ++set) {
+      uint64_t place = 0;
+      const uint64_t order = candidate(set, place);
+      const uint32_t high = uint32_t(order >> 32);
+      const uint32_t sorted = sorted_in_warp(high, lane);
+      if (lane == (num <= 32 ? num : 32) - 1) s_least[0][warp] = num <= 32 ? sorted : 0;
+      if (lane == (num + kSelWarps - 1) / kSelWarps - 1) s_least[1][warp] = sorted;
+      __syncthreads();
+      uint32_t most = 0, all = ~0u;
+#pragma unroll
+      for (int w = 0; w < kSelWarps; ++w) {
+        most = max(most, s_least[0][w]);
+        all = min(all, s_least[1][w]);
+      }
+      if (order && high >= max(most, all) && (order > least_order || (order == least_order && place < least_place))) {
+        const int n = atomicAdd(&s_n, 1);
+        s_order[n] = order;
+        s_place[n] = place;
       }
       __syncthreads();
-      const int n = s_n;
-      __syncthreads();
-      if (n + kSelThreads <= kJoinList && base + kSelThreads < all) continue;
-      for (int i = tid; i < n; i += kSelThreads) {
-        const uint64_t order = s_order[i], flat = s_flat[i];
-        int ahead = 0;
+      const int n = s_n, kept = least_order ? num : 0;
+      fresh = (parts > 1 && set % parts != 0 && fresh) || n > kept || !least_order;
+      if (n > kept) {
+        for (int i = tid; i < n; i += kSelThreads) {
+          const uint64_t o = s_order[i], q = s_place[i];
+          int ahead = 0;
 #pragma unroll 4
-        for (int k = 0; k < n; ++k) {
-          const uint64_t o = s_order[k];
-          ahead += o > order || (o == order && s_flat[k] < flat);
+          for (int k = 0; k < n; ++k) {
+            const uint64_t other = s_order[k];
+            ahead += other > o || (other == o && s_place[k] < q);
+          }
+          if (ahead < num) {
+            s_best[0][ahead] = o;
+            s_best[1][ahead] = q;
+          }
         }
-        if (ahead < num) {
-          s_best[0][ahead] = order;
-          s_best[1][ahead] = flat;
+        __syncthreads();
+        const int left = min(n, num);
+        if (tid < left) {
+          s_order[tid] = s_best[0][tid];
+          s_place[tid] = s_best[1][tid];
+        }
+        if (tid == 0) s_n = left;
+        if (left == num) {
+          least_order = s_best[0][num - 1];
+          least_place = s_best[1][num - 1];
         }
       }
       __syncthreads();
-      const int kept = min(n, num);
-      if (tid < kept) {
-        s_order[tid] = s_best[0][tid];
-        s_flat[tid] = s_best[1][tid];
-      }
-      if (tid == 0) s_n = kept;
-      if (kept == num) {
-        least_order = s_best[0][num - 1];
-        least_flat = s_best[1][num - 1];
-      }
-      __syncthreads();
+      if (!fresh && (parts == 1 || set % parts == parts - 1)) break;
     }
     if (again) break;
     // whether a candidate of another beam is too close to one that is chosen for 32 bits to tell them apart
     bool close = false;
     const double apart = too_close(V), edge = value_of(s_best[0][num - 1]) - apart;
-    for (int i = tid; i < all && !close; i += kSelThreads) {
-      uint64_t flat;
-      const uint64_t order = candidate(i, flat);
+    for (int set = 0; set < sets; ++set) {
+      uint64_t place = 0;
+      const uint64_t order = candidate(set, place);
       const double value = value_of(order);
-      if (!order || !(value > -INFINITY) || value < edge) continue;
-      const int k = i / each;
-      for (int r = 0; r < num; ++r) {
-        const double chosen = value_of(s_best[0][r]);
-        if (fabs(chosen - value) > apart) continue;
-        const int other = int(s_best[1][r] / uint64_t(V));
-        close = close || (other != k && (s_kind[other] == kOpen || s_kind[k] == kOpen));
+      const bool near = order && value > -INFINITY && value >= edge;
+      if (near) {
+        const int k = int(place >> 32);
+        for (int r = 0; r < num; ++r) {
+          const int other = int(s_best[1][r] >> 32);
+          if (fabs(value_of(s_best[0][r]) - value) > apart || other == k || (s_kind[other] != kOpen && s_kind[k] != kOpen)) continue;
+          close = true;
+          atomicOr(&s_close[k / 32], 1u << k % 32);
+          atomicOr(&s_close[other / 32], 1u << other % 32);
+        }
       }
+      if (parts == 1 && !__syncthreads_or(near)) break;
     }
     if (!__syncthreads_or(close)) break;
     for (int k = 0; k < beams; ++k) {
-      if (s_kind[k] != kOpen) continue;
+      if (s_kind[k] != kOpen || !(s_close[k / 32] >> k % 32 & 1u)) continue;
       const int64_t from = (g * beams + k) * stride;
       const double top = s_top[k];
       double sum = 0.;
@@ -344,13 +460,13 @@ beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ 
         s_total[k] = log(sum);
       }
     }
+    if (tid == 0) s_n = 0;
     __syncthreads();
   }
   if (tid < num) {
-    const uint64_t flat = s_best[1][tid];
     out_scores[g * num + tid] = float(value_of(s_best[0][tid]));
-    out_parents[g * num + tid] = int64_t(flat / uint64_t(V));
-    out_tokens[g * num + tid] = int64_t(flat % uint64_t(V));
+    out_parents[g * num + tid] = int64_t(s_best[1][tid] >> 32);
+    out_tokens[g * num + tid] = int64_t(uint32_t(s_best[1][tid]));
   }
 }
 
@@ -482,9 +598,17 @@ beam_reorder_kernel(const int64_t* __restrict__ slots, const int64_t* __restrict
 
 using namespace mb200;
 
+// Logits of a CTA: whole chunks, as many as leave about four CTAs for every SM.
+static int64_t slice_of(int64_t rows, int64_t V) {
+  const int64_t chunks = (V + kSelChunk - 1) / kSelChunk, wanted = int64_t(sm_count()) * 4 / (rows > 0 ? rows : 1);
+  const int64_t slices = wanted < 1 ? 1 : min64(wanted, chunks);
+  return (chunks + slices - 1) / slices * kSelChunk;
+}
+
 extern "C" int64_t mb200_beam_select_scratch_bytes(int64_t groups, int64_t beams, int64_t V, int num) {
-  if (groups < 0 || beams < 0 || V < 0 || num < 0) return 0;
-  return groups * beams * ((V + kSelSlice - 1) / kSelSlice) * int64_t(sizeof(Slice) + num * sizeof(uint64_t));
+  if (groups < 1 || beams < 1 || V < 1 || num < 1) return 0;
+  const int64_t slice = slice_of(groups * beams, V);
+  return groups * beams * ((V + slice - 1) / slice) * int64_t(sizeof(Slice) + num * sizeof(uint64_t));
 }
 
 extern "C" int mb200_beam_select(const void* logits, const float* scores, const uint8_t* finished, void* scratch, float* out_scores,
@@ -498,13 +622,13 @@ extern "C" int mb200_beam_select(const void* logits, const float* scores, const 
   if (!logits || !scores || !scratch || !out_scores || !out_tokens || !out_parents) return MB200_EINVAL;
   if (!aligned16(scratch)) return MB200_EALIGN;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t rows = groups * beams, n_slices = (V + kSelSlice - 1) / kSelSlice;
+  const int64_t rows = groups * beams, slice = slice_of(rows, V), n_slices = (V + slice - 1) / slice;
   if (beams * n_slices * num >= (int64_t(1) << 31)) return MB200_ETOOBIG;
   Slice* slices = static_cast<Slice*>(scratch);
   uint64_t* best = reinterpret_cast<uint64_t*>(slices + rows * n_slices);
   const dim3 grid(static_cast<unsigned>(n_slices), static_cast<unsigned>(rows));
   const bool vec = aligned16(logits) && row_stride * (dtype == MB200_F32 ? 4 : 2) % 16 == 0;
-#define MB200_SLICES(TT, VEC) beam_slices_kernel<TT, VEC><<<grid, kSelThreads, 0, st>>>((const TT*)logits, row_stride, int(V), num, slices, best)
+#define MB200_SLICES(TT, VEC) beam_slices_kernel<TT, VEC><<<grid, kSelThreads, 0, st>>>((const TT*)logits, row_stride, int(V), int(slice), num, slices, best)
   if (dtype == MB200_F32) { if (vec) MB200_SLICES(float, true); else MB200_SLICES(float, false); }
   else { if (vec) MB200_SLICES(__nv_bfloat16, true); else MB200_SLICES(__nv_bfloat16, false); }
 #undef MB200_SLICES
