@@ -294,3 +294,54 @@ def forward(self, x):
         xs = F.silu(self.conv1d(xs.transpose(1, 2))[:, :, :L].transpose(1, 2))
     y = ssm(self, xs, z)
     return self.out_proj(y)
+
+
+# ----------------------------------------------------------------- a block on packed sequences and on slots
+
+def packed_forward(self, x, cu_seqlens, cache=None, slots=None, resume=None, max_length=None):
+    """`forward` over sequences laid end to end: x (T, D) -> (T, D); cu_seqlens, slots, resume, max_length as in `selective_scan_packed`.
+
+    cache = (states (S, ED, N), windows (S, ED, 3)): pools in which the sequences leave, and may resume, their states, updated in place (under
+    torch.no_grad()).  Without it, and with gradients, the way to train on packed documents."""
+    states, windows = cache if cache is not None else (None, None)
+    xs, z = self.in_proj(x).chunk(2, dim=-1)
+    xs = causal_conv1d_silu_packed(xs, self.conv1d.weight, self.conv1d.bias, cu_seqlens=cu_seqlens, windows=windows, slots=slots, resume=resume)
+    A = -torch.exp(self.A_log.float())
+    delta, B, C = _project(self, xs)
+    delta = F.linear(delta, self.dt_proj.weight)
+    y = selective_scan_packed(xs, delta, A, B, C, self.D, z=z, delta_bias=self.dt_proj.bias, cu_seqlens=cu_seqlens, states=states, slots=slots,
+                              resume=resume, max_length=max_length)
+    return self.out_proj(y)
+
+
+def slot_step(self, x, cache, slots):
+    """`step` on pools: x (B, D) -> (B, D), row b's state and window in entry slots[b] of cache = (states, windows), updated in place."""
+    states, windows = cache
+    xs, z = self.in_proj(x).chunk(2, dim=1)
+    xc, _ = conv_step_fn(xs, windows, self.conv1d.weight, self.conv1d.bias, slots=slots)
+    A = -torch.exp(self.A_log.float())
+    delta, B, C = _project(self, xc)
+    delta = F.linear(delta, self.dt_proj.weight)
+    y, _ = ssm_step_fn(xc, states, delta, A, B, C, self.D, z=z, delta_bias=self.dt_proj.bias, slots=slots)
+    return self.out_proj(y)
+
+
+def _stack(self, x, mixer):
+    """The loop of `stack_forward` with `mixer(i, layer, normed)` in the place of the layers' own."""
+    h, res = x, None
+    for i, layer in enumerate(self.layers):
+        norm = layer.norm
+        normed, res = add_rms_norm(h, res, None if getattr(norm, "use_mup", False) else norm.weight, norm.eps)
+        h = mixer(i, layer, normed)
+    return _host().add_residual(h, res) if res is not None else h
+
+
+def stack_packed(self, x, cu_seqlens, caches=None, slots=None, resume=None, max_length=None):
+    """`packed_forward` through all layers of a stack (an object with `layers`, as the reference's Mamba); caches: one pair of pools a layer."""
+    return _stack(self, x, lambda i, layer, h: packed_forward(layer.mixer, h, cu_seqlens, None if caches is None else caches[i], slots, resume,
+                                                              max_length))
+
+
+def stack_slot_step(self, x, caches, slots):
+    """`slot_step` through all layers of a stack; x (B, D) -> (B, D)."""
+    return _stack(self, x, lambda i, layer, h: slot_step(layer.mixer, h, caches[i], slots))
