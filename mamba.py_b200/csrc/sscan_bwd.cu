@@ -258,7 +258,7 @@ sscan_bwd_tma_kernel(const __grid_constant__ BwdMaps maps, const SscanBwdParams 
           const float4 o = ((r & 1) ? op1 : op0)[r * (kBTE / 2)];
           const float2 Bp = *reinterpret_cast<const float2*>(sBC + r * (N / 2));
           const float2 dt = make_float2(o.x, o.y), dtx = make_float2(o.z, o.w);
-          const float2 e0v = __fmul2_rn(dt, A2[0]), e1v = __fmul2_rn(dt, A2[1]);
+          const float2 e0v = decay_exponent<kPacked>(dt, A2[0]), e1v = decay_exponent<kPacked>(dt, A2[1]);
           const float2 a0 = make_float2(ex2f(e0v.x), ex2f(e0v.y)), a1 = make_float2(ex2f(e1v.x), ex2f(e1v.y));
           h[0] = __ffma2_rn(a0, h[0], __fmul2_rn(dtx, make_float2(Bp.x, Bp.x)));
           h[1] = __ffma2_rn(a1, h[1], __fmul2_rn(dtx, make_float2(Bp.y, Bp.y)));
@@ -306,7 +306,7 @@ sscan_bwd_tma_kernel(const __grid_constant__ BwdMaps maps, const SscanBwdParams 
             dC[k] = fmaf(dy2.y, hcur.y, dy2.x * hcur.x);
             dB[k] = fmaf(g.y, dtx.y, g.x * dtx.x);
             gBs = k ? __ffma2_rn(g, Bv[k], gBs) : __fmul2_rn(g, Bv[k]);
-            const float2 ev = __fmul2_rn(dt, A2[k]);
+            const float2 ev = decay_exponent<kPacked>(dt, A2[k]);
             gc[k] = __fmul2_rn(make_float2(ex2f(ev.x), ex2f(ev.y)), g);
             const float2 w = __fmul2_rn(gc[k], hprev);
             dAacc[k] = __ffma2_rn(w, dt, dAacc[k]);

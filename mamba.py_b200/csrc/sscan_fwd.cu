@@ -120,16 +120,16 @@ template <typename T, int N, bool kWide = false> struct TmaFwdSmem {
 // With the S4D-real structure A[e, n] = (n + 1) A[e, 0] (the reference's initialisation,
 // mambapy/mamba.py:168-169) they are p, p r, p r^2, p r^3 with r = exp(delta A[e, 0]) and
 // p = exp(delta A[e, 4q]): two ex2 and three multiplies, which halves the load on the MUFU pipe.
-template <bool kStruct>
+template <bool kStruct, bool kPacked = false>
 __device__ __forceinline__ void decay4(float dl, const float2& A2lo, const float2& A2hi, float A0, float2& a_lo,
                                        float2& a_hi) {
   const float2 dd = make_float2(dl, dl);
   if constexpr (!kStruct) {
-    const float2 e_lo = __fmul2_rn(dd, A2lo), e_hi = __fmul2_rn(dd, A2hi);
+    const float2 e_lo = decay_exponent<kPacked>(dd, A2lo), e_hi = decay_exponent<kPacked>(dd, A2hi);
     a_lo = make_float2(ex2f(e_lo.x), ex2f(e_lo.y));
     a_hi = make_float2(ex2f(e_hi.x), ex2f(e_hi.y));
   } else {
-    const float2 e = __fmul2_rn(dd, make_float2(A0, A2lo.x));
+    const float2 e = decay_exponent<kPacked>(dd, make_float2(A0, A2lo.x));
     const float r = ex2f(e.x), p1 = ex2f(e.y);
     const float r2 = r * r;
     a_lo = make_float2(p1, p1 * r);
@@ -344,7 +344,7 @@ sscan_fwd_tma_kernel(const __grid_constant__ FwdMaps maps, const SscanFwdParams 
 #pragma unroll
           for (int i = 0; i < kCPT; ++i) {
             e.dxx[i] = make_float2(l.o[i].y, l.o[i].y);
-            decay4<kStruct>(l.o[i].x, A2lo[i], A2hi[i], A0[i], e.a_lo[i], e.a_hi[i]);
+            decay4<kStruct, kPacked>(l.o[i].x, A2lo[i], A2hi[i], A0[i], e.a_lo[i], e.a_hi[i]);
           }
           e.Bq = l.Bq; e.Cq = l.Cq;
           return e;
