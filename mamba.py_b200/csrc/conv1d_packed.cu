@@ -1,20 +1,19 @@
 // Depthwise causal conv1d + SiLU (d_conv = 4) over sequences of different lengths laid end to end, forward and backward:
 //     y[t,e] = silu( bias[e] + sum_k w[e,k] * in(t-3+k, e) ),   in = x within the sequence of row t,
-// and before its first row 0 or, when the sequence resumes, the window that its slot holds.  Streaming, bound by HBM as the kernels on
-// rectangles are (conv1d.cu, whose mapping this follows: a thread owns V channels and walks a chunk of rows with the last three inputs
-// in registers, the loads of a group of rows in flight together).
+// and before its first row 0 or, when the sequence resumes, the window that its slot holds.  Streaming: what it has to do is to read x and write y
+// once.
 //
-// Where sequences begin is a bit per row, which a CTA gathers from cu_seqlens into shared memory for its own rows: one round of loads for up
-// to as many sequences as it has threads.  A group of rows in which none begins, which is nearly all of them, takes a path without tests.
+// Where sequences begin is a bit per row.  Rows in front of which none begins, which is nearly all of them, take a path without tests.
 #include <type_traits>
 #include "conv1d.cuh"
 #include "packed.cuh"
+#include "tma.cuh"
 
 namespace mb200 {
 namespace {
 
 constexpr int kPkThreads = 256, kPkWarps = kPkThreads / 32, kPkResident = 3;
-constexpr int kPkChunk = 32, kPkGroup = 8;              // rows of a forward warp; rows whose loads go out together
+constexpr int kPkChunk = 32, kPkGroup = 8;              // rows of a warp; rows whose loads go out together
 
 // Both sigmoids of a pair from one reciprocal: 1 / (a b) times the other.  The exponentials stay below 2^60 for that (a sigmoid of less is 2^-60).
 // The special function unit, which takes 16 cycles for two results of a warp and was busy for 19 of 42 us at 8000 x 5120, has a quarter less to do.
@@ -56,15 +55,41 @@ __device__ __forceinline__ void load_window(const T* p, Pk<W> (&win)[V / W][kCon
     }
 }
 
+// The last three inputs of sequence r, whose first row is t, for V neighbouring channels; `old`: what is there counts.
+template <typename T, int V>
+__device__ __forceinline__ void leave_window(const Packed& seqs, int r, int t, bool old, const T* x, int64_t x_sl, T* at) {
+  const int n = seqs.end(r, t) - t;
+  T u[kConvK - 1][V];
+#pragma unroll
+  for (int k = 0; k < kConvK - 1; ++k) {
+    const int place = n - (kConvK - 1) + k;               // of the input that goes to entry k
+#pragma unroll
+    for (int i = 0; i < V; ++i) u[k][i] = Elem<T>::from_f(0.f);
+    if (place >= 0) {
+      const CVec<T, V> in = cload<T, V>(x + int64_t(t + place) * x_sl, true);
+#pragma unroll
+      for (int i = 0; i < V; ++i) u[k][i] = in.v[i];
+    } else if (old) {                                     // shorter than the window: what was there moves up
+#pragma unroll
+      for (int i = 0; i < V; ++i) u[k][i] = at[3 * i + n + k];
+    }
+  }
+  CVec<T, V> out[kConvK - 1];
+#pragma unroll
+  for (int j = 0; j < (kConvK - 1) * V; ++j) out[j / V].v[j % V] = u[j % 3][j / 3];
+#pragma unroll
+  for (int k = 0; k < kConvK - 1; ++k) cstore<T, V>(at + k * V, out[k]);
+}
+
 // The thread that meets a sequence's first row also leaves the window, when it is done with its rows: the only one that reads what the slot held.  So
 // the (at most two) rows after a first row that need it too, when they fall into the next chunk, are done by the chunk of the first row.
-// A warp finds out by itself which sequences begin in its rows, a lane a sequence, while the first rows and the filter are on their way: no
+// This form takes any strides, with one channel a thread; the tensor-map form below takes the others.  A warp finds out by itself which sequences begin in its rows, a lane a sequence, while the first rows and the filter are on their way: no
 // barrier, and for up to 32 sequences one load.
-template <typename T, int V>
+template <typename T>
 __global__ void __launch_bounds__(kPkThreads, kPkResident)
 conv1d_silu_packed_fwd_kernel(const Packed seqs, const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ bias,
                               T* __restrict__ y, T* windows, int64_t ED, int64_t x_sl, int64_t y_sl, int chunks) {
-  constexpr int kG = sizeof(T) * V > 8 ? kPkGroup / 2 : kPkGroup;
+  constexpr int V = 1, kG = kPkGroup;
   constexpr int kBefore = kConvK - 2, kSeen = kBefore + kPkChunk + kConvK - 2;
   struct Begins { int64_t slot; int seq; bool old; };     // a sequence, its slot or -1, and whether it resumes
   __shared__ Begins s_begins[kPkWarps][kSeen];
@@ -210,29 +235,171 @@ conv1d_silu_packed_fwd_kernel(const Packed seqs, const T* __restrict__ x, const 
       const int t = t0 + __ffsll(int64_t(own)) - 1;
       const Begins q = mine[t - t0 + kBefore];
       if (q.slot < 0) continue;
-      T* const at = windows + (q.slot * ED + e) * (kConvK - 1);
-      const int n = seqs.end(q.seq, t) - t;
-      T u[kConvK - 1][V];
+      leave_window<T, V>(seqs, q.seq, t, q.old, x + e, x_sl, windows + (q.slot * ED + e) * (kConvK - 1));
+    }
+  }
+}
+
+// The same for tensors that a tensor map describes.  With loads into registers a warp's are out only while it has nothing to compute, and neither the
+// instructions (36 % of the issue slots) nor HBM (half) are busy.  Here a warp does nothing but keep boxes of 32 rows (and the three in front,
+// the two behind) by 256 bytes of channels coming, several ahead, and finds where sequences begin in them; four warps take 8 rows of a box
+// each, a lane 8 bytes of channels, and store y.  A CTA walks through every gridDim.y-th box of its channels.
+// bfloat16, us so / one channel a thread / four: 8000 x 5120, 12 sequences 32.9 / - / 42.2 (a copy 27.4), 16000 x 1536 20.2 / 30.1 / 26.5, 4000 x 1536
+// 8.8 / 10.3 / 12.2, 2999 x 1000 7.4 / 6.9 / 9.4, 1000 x 512 4.2 / 5.0 / 9.1.
+constexpr int kTcRows = 32, kTcBox = kConvK - 1 + kTcRows + kConvK - 2, kTcBytes = 256, kTcStages = 4, kTcWarps = 4, kTcResident = 5;
+constexpr int kTcThreads = 32 * (kTcWarps + 1);
+
+__device__ int g_conv_status = MB200_DEV_OK;
+
+template <typename T>
+__global__ void __launch_bounds__(kTcThreads, kTcResident)
+conv1d_silu_packed_tma_kernel(const __grid_constant__ CUtensorMap map, const Packed seqs, const T* __restrict__ x,
+                              const float* __restrict__ w, const float* __restrict__ bias, T* __restrict__ y, T* windows,
+                              int64_t ED, int64_t x_sl, int64_t y_sl) {
+  constexpr int kTcChannels = kTcBytes / int(sizeof(T)), V = kTcChannels / 32, W = 2, P = V / W, kMine = kTcRows / kTcWarps, kBefore = kConvK - 2, kSeen = kBefore + kTcRows + kConvK - 2;
+  constexpr int kBytes = kTcBox * kTcBytes;
+  static_assert(kBytes % 128 == 0, "boxes stay aligned");
+  struct Begins { int64_t slot; int seq; bool old; };     // a sequence, its slot or -1, and whether it resumes
+  extern __shared__ __align__(128) unsigned char smem[];  // [kTcStages] boxes
+  __shared__ Begins s_begins[kTcStages][kSeen];
+  __shared__ uint64_t s_firsts[kTcStages];                // bit i: a sequence begins at row i - 2 of the box's 32
+  __shared__ uint64_t full[kTcStages], empty[kTcStages];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t e0 = int64_t(blockIdx.x) * kTcChannels;
+  const int boxes = (seqs.rows + kTcRows - 1) / kTcRows;
+  if (tid == 0) {
+#pragma unroll
+    for (int i = 0; i < kTcStages; ++i) { mbar_init(&full[i], 2); mbar_init(&empty[i], kTcWarps); }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  const int tail = seqs.start(seqs.sequences);            // rows from here on belong to no sequence
+  int stage = 0, round = 0;
+  auto next = [&]() {
+    if (++stage == kTcStages) { stage = 0; round ^= 1; }
+  };
+  if (warp == kTcWarps) {
+    int r0 = 0;                                           // sequences in front of it begin in front of the box
+    for (int box = blockIdx.y; box < boxes; box += gridDim.y) {
+      const int t0 = box * kTcRows;
+      if (!mbar_wait(&empty[stage], round ^ 1)) { atomicExch(&g_conv_status, MB200_DEV_WAIT_TIMEOUT); return; }
+      if (lane == 0) {
+        mbar_expect_tx(&full[stage], kBytes);
+        tma_load_3d(smem + stage * kBytes, &map, int(e0), t0 - (kConvK - 1), 0, &full[stage]);
+      }
+      for (;;) {
+        const int r = r0 + lane;
+        const int n = __popc(__ballot_sync(0xffffffffu, r < seqs.sequences && seqs.start(r) < t0 - kBefore));
+        r0 += n;
+        if (n < 32) break;
+      }
+      uint64_t firsts = 0;
+      for (int base = r0;; base += 32) {
+        const int r = base + lane, first = r < seqs.sequences ? seqs.start(r) : seqs.rows, at = first - t0 + kBefore;
+        const bool in = r < seqs.sequences && at >= 0 && at < kSeen;
+        if (in && seqs.end(r, first) > first) {
+          firsts |= uint64_t(1) << at;
+          s_begins[stage][at] = Begins{windows ? seqs.slot(r) : -1, r, seqs.resumes(r)};
+        }
+        if (!__all_sync(0xffffffffu, in)) break;          // (offsets that fall are nobody's promise)
+      }
+      firsts = uint64_t(__reduce_or_sync(0xffffffffu, unsigned(firsts))) | uint64_t(__reduce_or_sync(0xffffffffu, unsigned(firsts >> 32))) << 32;
+      if (lane == 0) {
+        s_firsts[stage] = firsts;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[stage]);
+      next();
+    }
+    return;
+  }
+  const int64_t e = e0 + lane * V;
+  const bool works = e < ED;
+  using F = Pk<W>;
+  F wk[P][kConvK], bv[P], win[P][kConvK - 1];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    bv[i] = works && bias ? F::load(bias + e + W * i, 1) : F::splat(0.f);
+#pragma unroll
+    for (int k = 0; k < kConvK; ++k) wk[i][k] = works ? F::load(w + (e + W * i) * kConvK + k, kConvK) : F::splat(0.f);
+  }
+  for (int box = blockIdx.y; box < boxes; box += gridDim.y) {
+    const int t0 = box * kTcRows + warp * kMine, t1 = min(t0 + kMine, seqs.rows);
+    if (!mbar_wait(&full[stage], round)) { atomicExch(&g_conv_status, MB200_DEV_WAIT_TIMEOUT); return; }
+    // row t of the box's; channel of this lane
+    const T* const in = reinterpret_cast<const T*>(smem + stage * kBytes) + (warp * kMine + kConvK - 1) * kTcChannels + lane * V;
+    auto at_row = [&](int i) { return *reinterpret_cast<const CVec<T, V>*>(in + i * kTcChannels); };
+    const uint64_t firsts = s_firsts[stage] >> (warp * kMine);             // bit i: row t0 - 2 + i
+    const Begins* const begins = s_begins[stage] + warp * kMine;
+    auto enter = [&](int i) {                             // the three rows in front of row i
 #pragma unroll
       for (int k = 0; k < kConvK - 1; ++k) {
-        const int place = n - (kConvK - 1) + k;             // of the input that goes to entry k
+        F xv[P];
+        unpack<T, V, W>(at_row(i + k - (kConvK - 1)), xv);
 #pragma unroll
-        for (int i = 0; i < V; ++i) u[k][i] = Elem<T>::from_f(0.f);
-        if (place >= 0) {
-          const CVec<T, V> in = cload<T, V>(x + int64_t(t + place) * x_sl + e, true);
+        for (int j = 0; j < P; ++j) win[j][k] = xv[j];
+      }
+    };
+    auto row = [&](const CVec<T, V>& q) {
+      F xn[P], o[P];
+      unpack<T, V, W>(q, xn);
 #pragma unroll
-          for (int i = 0; i < V; ++i) u[k][i] = in.v[i];
-        } else if (q.old) {                                 // shorter than the window: what was there moves up
+      for (int i = 0; i < P; ++i) {
+        F acc = pfma(wk[i][0], win[i][0], bv[i]);
+        acc = pfma(wk[i][1], win[i][1], acc);
+        acc = pfma(wk[i][2], win[i][2], acc);
+        acc = pfma(wk[i][3], xn[i], acc);
+        win[i][0] = win[i][1]; win[i][1] = win[i][2]; win[i][2] = xn[i];
+        o[i] = pmul(acc, psigmoid_pk(acc));
+      }
+      return pack<T, V, W>(o);
+    };
+    T* yp = y + int64_t(t0) * y_sl + e;
+    if (works && t0 + kMine <= tail && (firsts & ((uint64_t(1) << (kBefore + kMine)) - 1)) == 0) {
+      enter(0);
 #pragma unroll
-          for (int i = 0; i < V; ++i) u[k][i] = at[3 * i + n + k];
+      for (int j = 0; j < kMine; ++j) cstore<T, V>(yp + j * y_sl, row(at_row(j)));
+    } else if (works && t0 < seqs.rows) {
+      // as above: rows lo to hi are this warp's, and what begins among its 8 leaves its window here
+      auto first_at = [&](int i) { return (firsts >> (i + kBefore) & 1) != 0; };
+      const int n = t1 - t0, last = max(0, min(n, tail - t0));
+      int lo = 0, hi = last;
+      constexpr int kFar = -2 * kConvK;
+      const int in_front = first_at(-1) ? -1 : first_at(-2) ? -2 : kFar;
+      const int at_end = n != kMine ? kFar : first_at(n - 1) ? n - 1 : first_at(n - 2) ? n - 2 : kFar;
+      while (lo < n && lo - in_front < kConvK - 1 && !first_at(lo)) ++lo;
+      while (t0 + hi < tail && hi - at_end < kConvK - 1 && !first_at(hi)) ++hi;
+      enter(lo);
+#pragma unroll 1
+      for (int i = lo; i < hi; ++i) {
+        if (first_at(i)) {
+          const Begins q = begins[i + kBefore];
+          if (q.slot >= 0 && q.old) {
+            load_window<T, V, W>(windows + (q.slot * ED + e) * (kConvK - 1), win);
+          } else {
+#pragma unroll
+            for (int j = 0; j < P; ++j)
+#pragma unroll
+              for (int k = 0; k < kConvK - 1; ++k) win[j][k] = F::splat(0.f);
+          }
+        }
+        cstore<T, V>(yp + i * y_sl, row(at_row(i)));
+      }
+      CVec<T, V> zero;
+#pragma unroll
+      for (int i = 0; i < V; ++i) zero.v[i] = Elem<T>::from_f(0.f);
+      for (int i = last; i < n; ++i) cstore<T, V>(yp + i * y_sl, zero);
+      if (windows) {
+        for (uint64_t own = firsts >> kBefore & ((uint64_t(1) << kMine) - 1); own; own &= own - 1) {
+          const int i = __ffsll(int64_t(own)) - 1;
+          const Begins q = begins[i + kBefore];
+          if (q.slot >= 0) leave_window<T, V>(seqs, q.seq, t0 + i, q.old, x + e, x_sl, windows + (q.slot * ED + e) * (kConvK - 1));
         }
       }
-      CVec<T, V> out[kConvK - 1];
-#pragma unroll
-      for (int j = 0; j < (kConvK - 1) * V; ++j) out[j / V].v[j % V] = u[j % 3][j / 3];
-#pragma unroll
-      for (int k = 0; k < kConvK - 1; ++k) cstore<T, V>(at + k * V, out[k]);
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[stage]);
+    next();
   }
 }
 
@@ -391,6 +558,12 @@ int packed_chunk(int64_t rows, int64_t cols, int warps, int resident, int unit, 
   return best;
 }
 
+// Channels of a thread of the backward.  Four save instructions, one gives four times the warps: us with four / one, with the launches around it,
+//            1000 x 512   3000 x 1000   8000 x 512   4000 x 1536   2000 x 5120   8000 x 1536   16000 x 1536
+// float32     8.0 / 5.7    13.1 / 10.9    14.9 / 14.4  24.2 / 27.4   37.4 / 47.5   43.8 / 54.7   70.2 / 94.5
+// bfloat16    7.7 / 5.8    12.5 / 11.1    15.2 / 12.3  17.3 / 16.2   26.0 / 36.8   30.4 / 47.3   51.0 / 87.1
+bool one_channel(int64_t values, int dtype) { return values <= (dtype == MB200_F32 ? int64_t(9) << 19 : int64_t(7) << 20); }
+
 int check_conv(const mb200_packed* seqs, int64_t ED, int K, int dtype) {
   if (const int rc = packed_check(seqs)) return rc;
   if (ED < 0) return MB200_EINVAL;
@@ -403,23 +576,42 @@ int check_conv(const mb200_packed* seqs, int64_t ED, int K, int dtype) {
 
 using namespace mb200;
 
+// Reads (and clears) the device-side status word of the packed convolution.  Synchronises the device.
+int mb200_conv_device_status() {
+  int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_conv_status, sizeof(int)) != cudaSuccess) return -1;
+  if (v) cudaMemcpyToSymbol(g_conv_status, &zero, sizeof(int));
+  return v;
+}
+
 extern "C" int mb200_conv1d_silu_packed_fwd(const mb200_packed* seqs, const void* x, const float* w, const float* bias, void* windows, void* y,
                                             int64_t ED, int K, int64_t x_sl, int64_t y_sl, int dtype, void* stream) {
   if (const int rc = check_conv(seqs, ED, K, dtype)) return rc;
   if (seqs->rows == 0 || ED == 0) return MB200_OK;
   if (!x || !w || !y || (seqs->slots && !windows)) return MB200_EINVAL;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int kv = 4;
-  const bool vec = conv_vec_ok(ED, kv, {x, y, (const void*)windows}, {x_sl, y_sl});
-  const int v = vec ? kv : 1;
-  const int64_t cols = (ED + 32 * int64_t(v) - 1) / (32 * int64_t(v));
-  const int chunks = packed_chunk(seqs->rows, cols, kPkWarps, kPkResident, kPkChunk, 16 * kPkChunk, 16) / kPkChunk;
-  const dim3 grid(unsigned((seqs->rows + kPkWarps * kPkChunk * chunks - 1) / (kPkWarps * kPkChunk * chunks)), unsigned(cols));
   const Packed k = packed_of(*seqs, 0);
   if (!seqs->slots) windows = nullptr;
-#define MB200_CONV_FWD(TT, VV) conv1d_silu_packed_fwd_kernel<TT, VV><<<grid, kPkThreads, 0, st>>>(k, (const TT*)x, w, bias, (TT*)y, (TT*)windows, ED, x_sl, y_sl, chunks)
-  if (dtype == MB200_F32) { if (vec) MB200_CONV_FWD(float, 4); else MB200_CONV_FWD(float, 1); }
-  else { if (vec) MB200_CONV_FWD(__nv_bfloat16, 4); else MB200_CONV_FWD(__nv_bfloat16, 1); }
+  const bool bf = dtype == MB200_BF16;
+  const int channels = kTcBytes / (bf ? 2 : 4);
+  CUtensorMap map;
+  if (conv_vec_ok(ED, channels / 32, {x, y, (const void*)windows}, {y_sl}) && tma_compatible(x, 0, x_sl, ED, bf ? 2 : 4, channels) &&
+      tma_encode(&map, x, bf, 1, seqs->rows, ED, 0, x_sl, channels, kTcBox)) {
+    const int64_t across = (ED + channels - 1) / channels, boxes = (seqs->rows + kTcRows - 1) / kTcRows;
+    const int64_t down = int64_t(sm_count()) * kTcResident / across;
+    const dim3 walk(unsigned(across), unsigned(down < 1 ? 1 : min64(down, boxes)));
+#define MB200_CONV_FWD(TT) \
+  conv1d_silu_packed_tma_kernel<TT><<<walk, kTcThreads, kTcStages * kTcBox * kTcBytes, st>>>(map, k, (const TT*)x, w, bias, (TT*)y, (TT*)windows, ED, x_sl, y_sl)
+    if (bf) MB200_CONV_FWD(__nv_bfloat16); else MB200_CONV_FWD(float);
+#undef MB200_CONV_FWD
+    return check_launch();
+  }
+  const int64_t cols = (ED + 31) / 32;
+  const int chunks = packed_chunk(seqs->rows, cols, kPkWarps, kPkResident, kPkChunk, 16 * kPkChunk, 16) / kPkChunk;
+  const dim3 grid(unsigned((seqs->rows + kPkWarps * kPkChunk * chunks - 1) / (kPkWarps * kPkChunk * chunks)), unsigned(cols));
+#define MB200_CONV_FWD(TT) \
+  conv1d_silu_packed_fwd_kernel<TT><<<grid, kPkThreads, 0, st>>>(k, (const TT*)x, w, bias, (TT*)y, (TT*)windows, ED, x_sl, y_sl, chunks)
+  if (bf) MB200_CONV_FWD(__nv_bfloat16); else MB200_CONV_FWD(float);
 #undef MB200_CONV_FWD
   return check_launch();
 }
@@ -432,7 +624,7 @@ extern "C" int mb200_conv1d_silu_packed_bwd(const mb200_packed* seqs, const void
   if (!x || !w || !dy || !dx || !dw || seqs->slots) return MB200_EINVAL;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int kv = 4;
-  const bool vec = conv_vec_ok(ED, kv, {x, dy, (const void*)dx}, {x_sl, dy_sl, dx_sl});
+  const bool vec = !one_channel(seqs->rows * ED, dtype) && conv_vec_ok(ED, kv, {x, dy, (const void*)dx}, {x_sl, dy_sl, dx_sl});
   const int v = vec ? kv : 1;
   const int64_t cols = (ED + 32 * int64_t(v) - 1) / (32 * int64_t(v));
   const int chunk = packed_chunk(seqs->rows, cols, kPkBwdWarps, 4, 8, kPkBwdChunkMost, 16);

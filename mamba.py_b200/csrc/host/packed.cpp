@@ -335,6 +335,7 @@ Tensor conv1d_silu_packed(const Tensor& x, const Tensor& weight, const OptTensor
     check(mb200_conv1d_silu_packed_fwd(&s, ptr(xs), fptr(w32), fptr(b32), ptr(windows), ptr(y), W, int(K), st(xs, 0), st(y, 0), dtype_code(dt),
                                        cuda_stream()),
           "mb200_conv1d_silu_packed_fwd");
+    check_status("mb200_conv1d_silu_packed_fwd");
   }
   if (windows.defined()) written(windows);
   if (grad) {

@@ -175,3 +175,4 @@ int mb200_fwd_tma_try(const mb200::SscanFwdParams& p, int N, int dtype, cudaStre
 int mb200_fwd_device_status();
 int mb200_bwd_device_status();
 int mb200_block_step_device_status();
+int mb200_conv_device_status();

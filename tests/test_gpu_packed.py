@@ -232,6 +232,77 @@ def test_conv_gradients(lengths, W, dtype, with_bias):
         close(a, b, a.dtype, k)
 
 
+def _many_lengths(total, seed):
+    """Lengths of all kinds, so that first rows fall on every place of a box and of a warp's rows; the rest in one long sequence."""
+    g = torch.Generator().manual_seed(seed)
+    lengths = [1] * 20 + [2, 3, 0, 5] * 10 + torch.randint(1, 70, (60,), generator=g).tolist() + [0, 0, 255, 256, 257, 31, 32, 33]
+    return lengths + [total - sum(lengths)]
+
+
+def _fast_plain_conv(x, w, b, lengths, windows, slots, resume):
+    """In 64 bits on the GPU, all sequences at once: each row's taps from a line of heads and rows."""
+    W, R = x.shape[1], len(lengths)
+    x, w = x.double(), w.double()[:, 0]
+    heads = torch.zeros(R, 3, W, dtype=torch.float64, device=DEV)
+    ok = (slots >= 0) & (slots < len(windows)) & resume
+    heads[ok] = windows.double().transpose(1, 2)[slots[ok]]
+    parts, lo = [], 0
+    for r, n in enumerate(lengths):
+        parts += [heads[r], x[lo:lo + n]]
+        lo += n
+    line = torch.cat(parts)
+    taps = sum(line[k:line.shape[0] - 3 + k] * w[:, k] for k in range(4)) + b.double()
+    keep = torch.cat([torch.arange(n) + sum(lengths[:r]) + 3 * r for r, n in enumerate(lengths)]).to(DEV)
+    y = torch.cat([F.silu(taps[keep]), torch.zeros(x.shape[0] - lo, W, dtype=torch.float64, device=DEV)])
+    after = windows.clone()
+    at = 0
+    for r, n in enumerate(lengths):
+        if n and 0 <= int(slots[r]) < len(windows):
+            after[int(slots[r])] = line[at + n:at + n + 3].t().to(windows.dtype)
+        at += n + 3
+    return y, after
+
+
+@pytest.mark.parametrize("T,W,dtype", [(5300, 2048, torch.bfloat16), (9001, 1000, torch.bfloat16), (70001, 128, torch.bfloat16), (9000, 996, torch.bfloat16),
+                                       (4000, 5120, torch.bfloat16), (5000, 2048, torch.float32)])
+def test_conv_of_large_tensors(T, W, dtype):
+    """Above the sizes at which a thread takes several channels and boxes come through tensor maps (996: off their grid)."""
+    import mamba_b200
+    lengths = _many_lengths(T - 45, T)
+    R = len(lengths)
+    g = torch.Generator(device=DEV).manual_seed(T + W)
+    x, w, b = (torch.randn(*s, generator=g, device=DEV) for s in ((T, W), (W, 1, 4), (W,)))
+    x = x.to(dtype)
+    slots = torch.randperm(R + 2, generator=torch.Generator().manual_seed(R))[:R].to(DEV)
+    slots[4] = -1
+    resume = torch.rand(R, generator=g, device=DEV) < 0.7
+    windows = torch.randn(R + 2, W, 3, generator=g, device=DEV).to(dtype)
+    want, after = _fast_plain_conv(x, w, b, lengths, windows, slots, resume)
+    for _ in range(3):                                      # the same each time: nobody reads a window that is written already
+        pool = windows.clone()
+        with torch.no_grad():
+            y = mamba_b200.causal_conv1d_silu_packed(x, w, b, cu_seqlens=cu_of(lengths), windows=pool, slots=slots, resume=resume)
+        close(y, want, dtype, "y")
+        assert torch.equal(pool, after) and (y[T - 45:] == 0).all()
+
+
+@pytest.mark.parametrize("T,W,dtype", [(5300, 2048, torch.bfloat16), (5000, 1024, torch.float32), (9001, 996, torch.bfloat16)])
+def test_conv_gradients_of_large_tensors(T, W, dtype):
+    import mamba_b200
+    lengths = _many_lengths(T - 45, T)
+    g = torch.Generator(device=DEV).manual_seed(T + W)
+    t = [torch.randn(*s, generator=g, device=DEV) for s in ((T, W), (W, 1, 4), (W,))]
+    t[0] = t[0].to(dtype)
+    dy = torch.randn(T, W, generator=g, device=DEV).to(dtype)
+    leaves, exact = [v.clone().requires_grad_() for v in t], [v.double().requires_grad_() for v in t]
+    y = mamba_b200.causal_conv1d_silu_packed(*leaves, cu_seqlens=cu_of(lengths))
+    none = torch.full((len(lengths),), -1, device=DEV)
+    want, _ = _fast_plain_conv(*exact, lengths, torch.zeros(1, W, 3, device=DEV), none, none > 0)
+    close(y, want, dtype, "y")
+    for k, a, b in zip(("dx", "dw", "db"), torch.autograd.grad(y, leaves, dy), torch.autograd.grad(want, exact, dy.double())):
+        close(a, b, a.dtype, k)
+
+
 def test_conv_garbage_behind_and_across():
     import mamba_b200
     lengths, W = [21, 13, 40], 64
