@@ -454,22 +454,23 @@ typedef struct {
 /* mb200_sscan_fwd over packed sequences.  x, delta, z, y: (rows, ED), Bm, Cm: (rows, N); states: the pool (n_slots, ED, N) float32, read
  * and written in place, or NULL without slots.  carries (optional): mb200_packed_saved_states(rows, sequences) entries of ED x N floats for
  * mb200_sscan_packed_bwd.  piece_len > 0 (a multiple of 16; d_state 16, tensors that tensor maps describe, otherwise MB200_EUNSUPPORTED) cuts
- * sequences at every piece_len rows and scans the pieces side by side; pieces: 2 * mb200_packed_pieces(rows, sequences, piece_len) * ED * N floats. */
-int64_t mb200_packed_pieces(int64_t rows, int64_t sequences, int64_t piece_len);
+ * sequences at every piece_len rows and scans the pieces side by side, after a pass that computes what is carried through each of `parts` equal parts
+ * of a piece (1 or more, each a multiple of 16 rows); pieces: 2 * mb200_packed_parts(rows, sequences, piece_len / parts) * ED * N floats. */
+int64_t mb200_packed_parts(int64_t rows, int64_t sequences, int64_t part_len);
 int64_t mb200_packed_saved_states(int64_t rows, int64_t sequences);
 int mb200_sscan_packed_fwd(const mb200_packed* seqs, const void* x, const void* delta, const void* z, const float* A, const void* Bm,
                            const void* Cm, const float* D, const float* delta_bias, float* states, void* y, float* carries,
                            float* pieces, int64_t ED, int N, int64_t x_sl, int64_t d_sl, int64_t z_sl, int64_t b_sl,
-                           int64_t c_sl, int64_t y_sl, int64_t piece_len, int dtype, int flags, void* stream);
+                           int64_t c_sl, int64_t y_sl, int64_t piece_len, int64_t parts, int dtype, int flags, void* stream);
 
-/* mb200_sscan_bwd over packed sequences without slots.  carries, pieces, piece_len: as the forward left them; piece_grads: scratch of
- * mb200_packed_pieces(...) * ED * N floats.  dB, dC (rows, N), dA, dD, ddelta_bias: float32, ACCUMULATED into (caller zero-fills). */
+/* mb200_sscan_bwd over packed sequences without slots.  carries, pieces, piece_len, parts: as the forward had and left them; piece_grads: scratch of
+ * mb200_packed_parts(...) * ED * N floats.  dB, dC (rows, N), dA, dD, ddelta_bias: float32, ACCUMULATED into (caller zero-fills). */
 int mb200_sscan_packed_bwd(const mb200_packed* seqs, const void* x, const void* delta, const void* z, const float* A, const void* Bm,
                            const void* Cm, const float* D, const float* delta_bias, const void* dy, const float* carries,
                            const float* pieces, float* piece_grads, void* dx, void* ddelta, void* dz, float* dB, float* dC,
                            float* dA, float* dD, float* ddelta_bias, int64_t ED, int N, int64_t x_sl, int64_t d_sl, int64_t z_sl,
                            int64_t b_sl, int64_t c_sl, int64_t dy_sl, int64_t dx_sl, int64_t dd_sl, int64_t dz_sl,
-                           int64_t piece_len, int dtype, int flags, void* stream);
+                           int64_t piece_len, int64_t parts, int dtype, int flags, void* stream);
 
 /* mb200_conv1d_silu_fwd over packed sequences: taps before a sequence's first row are 0, or its slot's window if it resumes.  x, y: (rows, ED);
  * windows: the pool (n_slots, ED, 3) in the activations' type, oldest input first, left holding each sequence's last three inputs, or NULL

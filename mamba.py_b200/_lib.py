@@ -46,10 +46,10 @@ _SIGNATURES = {
     "mb200_carry_fold": (_int, [_ptr] * 3 + [_i64] * 2 + [_int, _int, _ptr]),
     "mb200_carry_fold_range": (_int, [_ptr] * 4 + [_i64] * 3 + [_int, _int, _int, _ptr]),
     "mb200_sscan_fwd_carry": (_int, [_ptr] * 7 + [_i64] * 3 + [_int] + [_i64] * 6 + [_int, _int, _ptr]),
-    "mb200_packed_pieces": (_i64, [_i64] * 3),
+    "mb200_packed_parts": (_i64, [_i64] * 3),
     "mb200_packed_saved_states": (_i64, [_i64] * 2),
-    "mb200_sscan_packed_fwd": (_int, [_ptr] * 13 + [_i64, _int] + [_i64] * 7 + [_int, _int, _ptr]),
-    "mb200_sscan_packed_bwd": (_int, [_ptr] * 21 + [_i64, _int] + [_i64] * 10 + [_int, _int, _ptr]),
+    "mb200_sscan_packed_fwd": (_int, [_ptr] * 13 + [_i64, _int] + [_i64] * 8 + [_int, _int, _ptr]),
+    "mb200_sscan_packed_bwd": (_int, [_ptr] * 21 + [_i64, _int] + [_i64] * 11 + [_int, _int, _ptr]),
     "mb200_conv1d_silu_packed_fwd": (_int, [_ptr] * 6 + [_i64, _int, _i64, _i64, _int, _ptr]),
     "mb200_conv1d_silu_packed_bwd": (_int, [_ptr] * 8 + [_i64, _int] + [_i64] * 3 + [_int, _ptr]),
     "mb200_ssm_step_slots": (_int, [_ptr] * 4 + [_int, _int] + [_ptr] * 3 + [_int, _ptr, _int, _ptr, _ptr, _i64, _ptr, _i64, _i64, _int]

@@ -258,6 +258,5 @@ void selftest_queue_conversions(int64_t n);
 void selftest_block_step_give_up(const Tensor& on);
 
 int64_t pick_pieces(int64_t batch, int64_t length, int64_t width, bool grad);
-int64_t pick_piece_length(int64_t rows, int64_t sequences, int64_t longest, int64_t width, bool grad);
 
 }  // namespace mb200_host

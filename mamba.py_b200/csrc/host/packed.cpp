@@ -65,13 +65,13 @@ bool on_grid(const Tensor& t) {
 struct PackedScan {
   Tensor x, delta, A, B, C, D, z, bias;
   Sequences seqs;
-  int64_t piece_len = 0;
+  int64_t piece_len = 0, parts = 1;
   int flags() const { return (bias.defined() ? MB200_DELTA_SOFTPLUS : 0) | MB200_PAIRED_STATES; }
   int code() const { return dtype_code(x.scalar_type()); }
   int64_t rows() const { return x.size(0); }
   int64_t width() const { return x.size(1); }
   int64_t states() const { return A.size(1); }
-  int64_t pieces() const { return mb200_packed_pieces(rows(), seqs.count(), piece_len); }
+  int64_t n_parts() const { return mb200_packed_parts(rows(), seqs.count(), piece_len / parts); }
   bool maps() const {
     return on_grid(x) && on_grid(delta) && on_grid(z) && on_grid(B) && on_grid(C) && width() * x.element_size() % 16 == 0;
   }
@@ -97,7 +97,7 @@ struct PackedScanBackward : public torch::autograd::Node {
   Saved x, delta, A, B, C, D, z, bias, cu, carries, pieces;
   at::ScalarType types[kInputs];
   bool given[kInputs];
-  int64_t piece_len = 0;
+  int64_t piece_len = 0, parts = 1;
 
   std::string name() const override { return "PackedSelectiveScanBackward"; }
   void release_variables() override {
@@ -111,6 +111,7 @@ struct PackedScanBackward : public torch::autograd::Node {
     a.seqs.cu = cu.get();
     a.seqs.rows = a.rows();
     a.piece_len = piece_len;
+    a.parts = parts;
     const c10::cuda::CUDAGuard guard(a.x.device());
     const auto dt = a.x.scalar_type();
     Tensor dy = rows(grads[0], dt);
@@ -121,12 +122,12 @@ struct PackedScanBackward : public torch::autograd::Node {
     zero_fill(acc);
     const Tensor dB = alias(acc, 0, {T, N}), dC = alias(acc, T * N, {T, N}), dA = alias(acc, 2 * T * N, {W, N}),
                  dD = alias(acc, 2 * T * N + W * N, {W}), db = a.bias.defined() ? alias(acc, 2 * T * N + W * N + W, {W}) : Tensor();
-    const Tensor pg = piece_len ? empty({a.pieces(), W, N}, at::kFloat, a.x) : Tensor(), car = carries.get(), pcs = pieces.get();
+    const Tensor pg = piece_len ? empty({a.n_parts(), W, N}, at::kFloat, a.x) : Tensor(), car = carries.get(), pcs = pieces.get();
     const mb200_packed s = a.seqs.abi();
     check(mb200_sscan_packed_bwd(&s, ptr(a.x), ptr(a.delta), ptr(a.z), fptr(a.A), ptr(a.B), ptr(a.C), fptr(a.D), fptr(a.bias), ptr(dy), fptr(car),
                                  fptr(pcs), fptr(pg), ptr(dx), ptr(dd), ptr(dz), fptr(dB), fptr(dC), fptr(dA), fptr(dD), fptr(db), W, int(N),
                                  st(a.x, 0), st(a.delta, 0), st(a.z, 0), st(a.B, 0), st(a.C, 0), st(dy, 0), st(dx, 0), st(dd, 0), st(dz, 0),
-                                 piece_len, a.code(), a.flags(), cuda_stream()),
+                                 piece_len, parts, a.code(), a.flags(), cuda_stream()),
           "mb200_sscan_packed_bwd");
     check_status("mb200_sscan_packed_bwd");
     const Tensor all[kInputs] = {dx, dd, dA, dB, dC, dD, dz, db};
@@ -181,19 +182,32 @@ struct PackedConvBackward : public torch::autograd::Node {
 
 }  // namespace
 
-// Where to cut sequences (0: nowhere), from a model of the time of the passes, as pick_pieces has it for rows of one length and with its
-// measured times for 2048 rows with 1 / 2 / 3 CTAs on every SM.  Lengths are known to the device alone: one sequence is taken to be `longest`,
-// the others to share the rest evenly.  A pass takes the longer of
+// Where to cut sequences (length 0: nowhere), and into how many parts a piece goes for the carry passes, from a model of the time of the passes, as
+// pick_pieces has it for rows of one length and with its measured times for 2048 rows with 1 / 2 / 3 CTAs on every SM.  Lengths are known to the
+// device alone: one sequence is taken to be `longest`, the others to share the rest evenly.  A pass takes the longer of
 //   all its CTAs' rows at the rate of as many CTAs as there are on an SM;
 //   its whole pieces in rounds, the others in the gaps (a tenth more of them than there are if others compete: the longest do not spread
 //     over the SMs evenly then, six SMs of 148 had two while ten had none);
 //   with few whole pieces: the others, and then what is left of the whole ones at the pace of an SM of their own.
-// Over 40 cases (1 to 64 sequences, 325 to 16384 rows, 32 to 5120 channels, both types, training and serving) the length picked takes 2.0 %
-// longer than the best of 13 on average and 15 % at most; not cutting takes up to 15 times as long (one sequence of 16384 x 256: 616 us for 70).
-int64_t pick_piece_length(int64_t rows, int64_t sequences, int64_t longest, int64_t width, bool grad) {
+// The parts are as many as give the carry passes three CTAs on every SM, four at most and 48 rows at least: those passes go through pieces of the cut
+// sequences alone, and waited for few long ones.
+// Over 60 cases (1 to 64 sequences, 325 to 16384 rows, 32 to 5120 channels, both types, training and serving) the cut picked takes 3.6 % longer than the
+// best of 13 on average and 16 % at most; not cutting takes up to nine times as long (one sequence of 16384 x 256: 616 us for 70).  Parts took 16384 rows
+// of 1536 in 20 documents from 870 to 793 us of training, one sequence of 14213 among others from 291 to 267 of reading.
+struct Cut { int64_t length, parts; };
+constexpr int64_t kShortestPart = 48, kMostParts = 4;
+
+static int64_t parts_of(int64_t piece, double whole, double tiles, double sms) {
+  int64_t parts = std::min<int64_t>(kMostParts, std::max<int64_t>(1, int64_t(std::ceil(3 * sms / std::max(1.0, whole * tiles)))));
+  while (parts > 1 && (piece % (16 * parts) || piece / parts < kShortestPart)) --parts;
+  return parts;
+}
+
+// `piece`: a length to be taken as it is, or -1.
+static Cut pick_cut(int64_t rows, int64_t sequences, int64_t longest, int64_t width, bool grad, int64_t piece = -1) {
   constexpr double kFill = 20, kFwdSaving[] = {0, 82, 123, 174}, kFwd[] = {0, 79, 121, 170}, kBwd[] = {0, 279, 378, 538},
                    kFwdCarry[] = {0, 55, 87, 125}, kBwdCarry[] = {0, 62, 94, 135};
-  if (rows <= 0 || sequences <= 0 || longest <= 0) return 0;
+  if (rows <= 0 || sequences <= 0 || longest <= 0 || piece == 0) return {0, 1};
   const double sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount, tiles = double((width + 31) / 32);
   const double rest = sequences > 1 ? double(std::max<int64_t>(rows - longest, 0)) / double(sequences - 1) : 0;
   struct Group { double length, count; };
@@ -215,31 +229,37 @@ int64_t pick_piece_length(int64_t rows, int64_t sequences, int64_t longest, int6
     double us = std::max(n >= sms ? work / sms * step(c) / c : 0.0, (most + kFill) * (per_sm / 3 * step(3) + step(per_sm % 3)));
     if (full <= 2 * sms && n > full) {
       const double others = (work - full_work) / sms * step(3) / 3 / (1 - std::min(0.9, full / sms / 3));
-      us = std::max(us, others + (most - others / step(3)) * step(full <= sms ? 1 : 2));
+      us = std::max(us, others + (most - others / step(3)) * step(1.2 * full <= sms ? 1 : 2));
     }
     return us;
   };
-  int64_t best = 0;
+  Cut best{0, 1};
   double best_us = 0;
   for (const int64_t S : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48}) {
-    const int64_t P = (longest + 16 * S - 1) / (16 * S) * 16;
-    if (S > 1 && P < 64) break;
+    int64_t P = piece > 0 ? piece : (longest + 16 * S - 1) / (16 * S) * 16;
+    if (piece < 0 && P >= 2 * 64) P = (P + 63) / 64 * 64;               // (divisible into parts)
+    if (piece < 0 && S > 1 && P < 64) break;
     Group main[4] = {}, carry[4] = {};
     int k = 1;
     double whole = 0;
     for (const Group& q : {Group{double(longest), 1}, Group{rest, double(sequences - 1)}}) {
       if (q.length <= 0 || q.count <= 0) continue;
-      const double pieces = S > 1 ? std::ceil(q.length / double(P)) : 1;
+      const double pieces = S > 1 || piece > 0 ? std::ceil(q.length / double(P)) : 1;
       whole += q.count * (pieces - 1);
       main[k++] = Group{q.length - (pieces - 1) * double(P), q.count};
     }
-    main[0] = carry[0] = Group{double(P), whole};
+    const int64_t parts = parts_of(P, whole, tiles, sms);
+    if (piece > 0) return {P, parts};
+    main[0] = Group{double(P), whole};
+    carry[0] = Group{double(P) / double(parts), whole * double(parts)};
     double us = pass(main, grad ? kFwdSaving : kFwd) + (grad ? pass(main, kBwd) : 0);
     if (whole > 0) us += pass(carry, kFwdCarry) + (grad ? pass(carry, kBwdCarry) : 0) + (grad ? 16 : 7);
+    if (whole > 0 && sequences > 2) us *= 1.1;                          // the others are not even, and more of them will be cut
     if (S == 1 || us < best_us) {
-      best = S == 1 ? 0 : P;
+      best = S == 1 ? Cut{0, 1} : Cut{P, parts};
       best_us = us;
     }
+    if (S == 1 && us < (grad ? 24 : 12)) break;                         // nothing to gain, and 1 us of the host's to lose
   }
   return best;
 }
@@ -277,15 +297,18 @@ Tensor selective_scan_packed(const Tensor& x, const Tensor& delta, const Tensor&
                    Sequences(x, cu, states, slots, resume)};
     align_bc(a);
     const int64_t R = a.seqs.count(), longest = std::min(T, max_length.value_or(T));
-    if (N == 16 && a.maps() && T > 0) a.piece_len = piece_length ? *piece_length : pick_piece_length(T, R, longest, W, grad);
-    if (a.piece_len >= longest) a.piece_len = 0;
+    if (N == 16 && a.maps() && (!piece_length || *piece_length < longest)) {
+      const Cut cut = pick_cut(T, R, longest, W, grad, piece_length.value_or(-1));
+      a.piece_len = cut.length < longest ? cut.length : 0;
+      a.parts = a.piece_len ? cut.parts : 1;
+    }
     y = empty({T, W}, dt, a.x);
     if (grad) carries = empty({mb200_packed_saved_states(T, R), W, N}, at::kFloat, a.x);
-    if (a.piece_len) pieces = empty({2, a.pieces(), W, N}, at::kFloat, a.x);
+    if (a.piece_len) pieces = empty({2, a.n_parts(), W, N}, at::kFloat, a.x);
     const mb200_packed s = a.seqs.abi();
     check(mb200_sscan_packed_fwd(&s, ptr(a.x), ptr(a.delta), ptr(a.z), fptr(a.A), ptr(a.B), ptr(a.C), fptr(a.D), fptr(a.bias), fptr(states), ptr(y),
                                  fptr(carries), fptr(pieces), W, int(N), st(a.x, 0), st(a.delta, 0), st(a.z, 0), st(a.B, 0), st(a.C, 0), st(y, 0),
-                                 a.piece_len, a.code(), a.flags(), cuda_stream()),
+                                 a.piece_len, a.parts, a.code(), a.flags(), cuda_stream()),
           "mb200_sscan_packed_fwd");
     check_status("mb200_sscan_packed_fwd");
   }
@@ -300,7 +323,7 @@ Tensor selective_scan_packed(const Tensor& x, const Tensor& delta, const Tensor&
     node->set_next_edges(torch::autograd::collect_next_edges(x, delta, A, B, C, D, z, bias));
     node->x.save(a.x); node->delta.save(a.delta); node->A.save(a.A); node->B.save(a.B); node->C.save(a.C); node->D.save(a.D);
     node->z.save(a.z); node->bias.save(a.bias); node->cu.save(a.seqs.cu); node->carries.save(carries); node->pieces.save(pieces);
-    node->piece_len = a.piece_len;
+    node->piece_len = a.piece_len; node->parts = a.parts;
     torch::autograd::set_history(y, node);
   }
   return y;

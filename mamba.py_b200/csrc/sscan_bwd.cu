@@ -87,7 +87,7 @@ __device__ __forceinline__ void red_add_v4(float* addr, float a, float b, float 
 // (Without a gate the sum for y, which only dz needs, is still formed and handed over: 501 us for 525 on 8 x 2048 x 1536 in bfloat16.)
 // Saved states that lie next to a channel's others instead of two by two are 8-byte loads 64 bytes apart: 556 us there for 525, 138 for 134
 // on 3 x 1003 x 1000.
-// kPacked: the grid's second dimension numbers the pieces of packed sequences, as in the forward; a piece folds the carries of those behind it.
+// kPacked: the grid's second dimension numbers the pieces of packed sequences, as in the forward; a piece folds the carries of the parts behind it.
 template <typename T, bool kRev, bool kSoftplus, bool kHasZ, bool kPacked = false>
 __global__ void __launch_bounds__(kBwdThreads, 3)
 sscan_bwd_tma_kernel(const __grid_constant__ BwdMaps maps, const SscanBwdParams p) {
@@ -185,8 +185,9 @@ sscan_bwd_tma_kernel(const __grid_constant__ BwdMaps maps, const SscanBwdParams 
         dAacc[k] = make_float2(0.f, 0.f);
       }
       if constexpr (kPacked) {
-        const int last = item.first + item.pieces - 1;
-        for (int k = last; k > item.first + pc; --k) {
+        const int last = item.first_part + item.n_parts - 1;
+#pragma unroll 1
+        for (int k = last; k >= item.first_part + (pc + 1) * p.seqs.parts; --k) {
           const int64_t at = (k * p.ED + e) * N + n0;
           auto get = [&](const float* from, bool ok, int64_t more) { return ok ? *reinterpret_cast<const float2*>(from + at + more) : make_float2(0.f, 0.f); };
           const float2 G0 = get(p.pieceG, ok0, 0), G1 = get(p.pieceG, ok1, N);
@@ -712,9 +713,9 @@ extern "C" int mb200_sscan_packed_bwd(const mb200_packed* seqs, const void* x, c
                                       const float* pieces, float* piece_grads, void* dx, void* ddelta, void* dz, float* dB, float* dC,
                                       float* dA, float* dD, float* ddelta_bias, int64_t ED, int N, int64_t x_sl, int64_t d_sl, int64_t z_sl,
                                       int64_t b_sl, int64_t c_sl, int64_t dy_sl, int64_t dx_sl, int64_t dd_sl, int64_t dz_sl,
-                                      int64_t piece_len, int dtype, int flags, void* stream) {
+                                      int64_t piece_len, int64_t parts, int dtype, int flags, void* stream) {
   if (const int rc = packed_check(seqs)) return rc;
-  if (ED < 0 || piece_len < 0 || piece_len % kBTile) return MB200_EINVAL;
+  if (ED < 0 || piece_len < 0 || parts < 1 || piece_len % (parts * kBTile)) return MB200_EINVAL;
   if (dtype != MB200_F32 && dtype != MB200_BF16) return MB200_EDTYPE;
   if (N != 8 && N != 16 && N != 32 && N != 64) return MB200_ENSTATE;
   if (seqs->rows == 0 || ED == 0) return MB200_OK;
@@ -731,7 +732,7 @@ extern "C" int mb200_sscan_packed_bwd(const mb200_packed* seqs, const void* x, c
   p.B = 1; p.L = seqs->rows; p.ED = ED;
   p.x_sl = x_sl; p.d_sl = d_sl; p.z_sl = z_sl; p.b_sl = b_sl; p.c_sl = c_sl; p.dy_sl = dy_sl; p.dx_sl = dx_sl; p.dd_sl = dd_sl; p.dz_sl = dz_sl;
   p.flags = flags & (MB200_DELTA_SOFTPLUS | MB200_GENERAL_DECAY | MB200_PAIRED_STATES);
-  p.seqs = packed_of(*seqs, piece_len);
+  p.seqs = packed_of(*seqs, piece_len, parts);
   p.pieceP = pieces; p.pieceG = piece_grads;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int es = dtype == MB200_F32 ? 4 : 2;

@@ -158,10 +158,11 @@ __device__ __forceinline__ bool s4d_structured(const float* a4, float a0, int q)
 // p.carries (a template parameter because the test alone costs the recurrence warps 3 % of a prompt and 4 to 14 % of a carry pass:
 // 78.3 -> 80.9 us for 2048 steps of one CTA per SM, 52.7 -> 59.9 for 23 of 24 pieces of 53013 x 64).  Without y and kSave it is a carry pass,
 // which returns every piece's state; without y but with kSave a scan, which returns a row's last and saves states if there is p.carries.
-// kPacked: the grid's second dimension numbers the pieces of the packed sequences `p.seqs`.  A box that reaches past a piece's last row
+// kPacked: the grid's second dimension numbers the pieces of the packed sequences `p.seqs`, or, in the carry passes, their parts: those are few, being
+// in cut sequences alone, and shorter ones spread over the SMs.  A box that reaches past a piece's last row
 // then holds rows of the next sequence, whose values the converter drops (0 * NaN would not).  The first piece of a cut sequence enters from
 // the slot in the carry pass already, which keeps what the slot held for the first piece of the scan (the last one may have written
-// the slot by then) in the place of the last piece's carry, which nobody needs.  The scan folds the carries of the pieces in front
+// the slot by then) in the place of the last part's carry, which nobody needs.  The scan folds the carries of the pieces in front
 // of its own as it starts: a few loads in flight together, where a launch of their own takes 4 us.
 template <typename T, int N, bool kRev, bool kCarry, bool kHasY, bool kSave, bool kWide = false, bool kPacked = false>
 __global__ void __launch_bounds__(FwdGeom<N, kWide>::kThreads, FwdGeom<N, kWide>::kOcc)
@@ -188,13 +189,14 @@ sscan_fwd_tma_kernel(const __grid_constant__ FwdMaps maps, const SscanFwdParams 
   const int64_t e0 = int64_t(blockIdx.x) * kTE;
   const int64_t b = kPacked ? 0 : blockIdx.y;
   PackedItem item{};
-  if constexpr (kPacked) item = packed_item<G::kThreads>(p.seqs, int(blockIdx.y), tid);
+  if constexpr (kPacked)
+    item = packed_item<G::kThreads>(p.seqs, int(blockIdx.y), tid, kHasY ? kPieces : kCarry ? kPartsBehind : kSave ? kPartsButLast : kPartsBefore);
   const int pc = kPacked ? item.pc : int(blockIdx.z + p.piece0), t_lo = kPacked ? item.lo : int(pc * p.piece_len),
             t_hi = kPacked ? item.hi : int(min64(p.L, t_lo + p.piece_len));
-  const int64_t slot = kPacked ? int64_t(item.first + pc) : b * p.pieces + pc;
+  const int64_t slot = kPacked ? int64_t(item.first_part + pc) : b * p.pieces + pc;
   const int cols_ok = int(min64(kTE, p.ED - e0));
   const bool softplus = (p.flags & MB200_DELTA_SOFTPLUS) != 0;
-  constexpr bool has_y = kHasY, kEvery = !kHasY && !kSave;
+  constexpr bool has_y = kHasY, kEvery = !kHasY && (kPacked || !kSave);
   const bool has_z = p.z != nullptr;
   const int ntiles = (t_hi - t_lo + kTile - 1) / kTile;
   int64_t pool = -1;                                      // this sequence's slot
@@ -203,7 +205,7 @@ sscan_fwd_tma_kernel(const __grid_constant__ FwdMaps maps, const SscanFwdParams 
       if (has_y) zero_rows<T, G::kThreads>(static_cast<T*>(p.y) + e0, p.y_sl, t_lo, t_hi, cols_ok, tid);
       return;
     }
-    if (ntiles == 0 || (kEvery && pc == (kCarry ? 0 : item.pieces - 1))) return;       // no rows; nothing follows (precedes) the last (first) piece
+    if (ntiles == 0) return;
     pool = p.seqs.slot(item.seq);
   }
   // Direction.  With MB200_REVERSE time is walked from L-1 down to 0: processing tile kt is the
@@ -256,15 +258,15 @@ sscan_fwd_tma_kernel(const __grid_constant__ FwdMaps maps, const SscanFwdParams 
           auto get = [&](const float* from, int64_t k) { return *reinterpret_cast<const float4*>(from + k * each + at); };
           if (pc == 0) {
             if (pool >= 0 && p.seqs.resumes(item.seq)) {
-              const int64_t kept = item.first + item.pieces - 1;
+              const int64_t kept = item.first_part + item.n_parts - 1;
               const bool cut = item.pieces > 1;
               put(!kEvery && cut ? get(p.pieceS, kept) : get(p.h0, pool));
               if (kEvery && cut) *reinterpret_cast<float4*>(p.pieceS + kept * each + at) = make_float4(h4[0], h4[1], h4[2], h4[3]);
             }
           } else if constexpr (!kEvery) {
-            put(get(p.pieceS, item.first));
+            put(get(p.pieceS, item.first_part));
 #pragma unroll 4
-            for (int k = item.first + 1; k < item.first + pc; ++k) {
+            for (int k = item.first_part + 1; k < item.first_part + pc * p.seqs.parts; ++k) {
               const float4 P = get(p.pieceP, k), S = get(p.pieceS, k);
               put(make_float4(fmaf(P.x, h4[0], S.x), fmaf(P.y, h4[1], S.y), fmaf(P.z, h4[2], S.z), fmaf(P.w, h4[3], S.w)));
             }
@@ -360,7 +362,7 @@ sscan_fwd_tma_kernel(const __grid_constant__ FwdMaps maps, const SscanFwdParams 
         for (int t = 0; t < kDecayAhead; ++t) rd[t] = prepare(ld[t]);
 #pragma unroll
         for (int t = 0; t < kTile; ++t) {
-          if (kSave && t % kChunk == 0 && (kHasY || p.carries)) {            // state entering this chunk
+          if (kSave && (kHasY || !kPacked) && t % kChunk == 0 && (kHasY || p.carries)) {            // state entering this chunk
             if (t0a + (rev ? kChunk - t : t) < (kPacked ? t_hi : p.L)) {
 #pragma unroll
               for (int i = 0; i < kCPT; ++i) {
@@ -647,7 +649,8 @@ sscan_fwd_tma_kernel(const __grid_constant__ FwdMaps maps, const SscanFwdParams 
   }
 }
 
-// The packed forms: the scan, with and without saved states, and (d_state 16, where sequences are cut) the two carry passes.
+// The packed forms: the scan, with and without saved states, and (d_state 16, where sequences are cut) the carry passes: the forward one of a scan
+// that saves states leaves the decay products of a few parts more, which the backward needs.
 template <typename T, int N, bool kWide>
 int tma_launch_packed(const FwdMaps& m, const SscanFwdParams& p, bool every, cudaStream_t st) {
   using G = FwdGeom<N, kWide>;
@@ -656,10 +659,11 @@ int tma_launch_packed(const FwdMaps& m, const SscanFwdParams& p, bool every, cud
       p.carries ? sscan_fwd_tma_kernel<T, N, false, false, true, true, kWide, true> : sscan_fwd_tma_kernel<T, N, false, false, true, false, kWide, true>;
   if constexpr (N == 16 && !kWide) {
     if (every) k = p.flags & kFlagCarryPass ? sscan_fwd_tma_kernel<T, N, true, true, false, false, false, true>
+                   : p.carries              ? sscan_fwd_tma_kernel<T, N, false, false, false, true, false, true>
                                             : sscan_fwd_tma_kernel<T, N, false, false, false, false, false, true>;
   }
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess) return MB200_ELAUNCH;
-  const int64_t items = packed_items(p.seqs.rows, p.seqs.sequences, p.seqs.piece);
+  const int64_t items = packed_items(p.seqs.rows, p.seqs.sequences, every ? p.seqs.piece / p.seqs.parts : p.seqs.piece);
   if (items > 65535) return MB200_ETOOBIG;
   k<<<dim3(unsigned((p.ED + G::kTE - 1) / G::kTE), unsigned(items)), G::kThreads, S::kBytes, st>>>(m, p);
   return check_launch();
@@ -879,18 +883,17 @@ extern "C" int mb200_sscan_fwd_carry(const void* x, const void* delta, const flo
                                       1, 0, stream);
 }
 
-// The pieces of cut sequences come from the carry pass in front of the scan, both in one call.
-extern "C" int64_t mb200_packed_pieces(int64_t rows, int64_t sequences, int64_t piece_len) {
-  return piece_len > 0 ? packed_items(rows, sequences, piece_len) : 0;
+extern "C" int64_t mb200_packed_parts(int64_t rows, int64_t sequences, int64_t part_len) {
+  return part_len > 0 ? packed_items(rows, sequences, part_len) : 0;
 }
 extern "C" int64_t mb200_packed_saved_states(int64_t rows, int64_t sequences) { return packed_chunks(rows, sequences, kChunk); }
 
 extern "C" int mb200_sscan_packed_fwd(const mb200_packed* seqs, const void* x, const void* delta, const void* z, const float* A, const void* Bm,
                                       const void* Cm, const float* D, const float* delta_bias, float* states, void* y, float* carries,
                                       float* pieces, int64_t ED, int N, int64_t x_sl, int64_t d_sl, int64_t z_sl, int64_t b_sl,
-                                      int64_t c_sl, int64_t y_sl, int64_t piece_len, int dtype, int flags, void* stream) {
+                                      int64_t c_sl, int64_t y_sl, int64_t piece_len, int64_t parts, int dtype, int flags, void* stream) {
   if (const int rc = packed_check(seqs)) return rc;
-  if (ED < 0 || piece_len < 0 || piece_len % kTile) return MB200_EINVAL;
+  if (ED < 0 || piece_len < 0 || parts < 1 || piece_len % (parts * kTile)) return MB200_EINVAL;
   if (dtype != MB200_F32 && dtype != MB200_BF16) return MB200_EDTYPE;
   if (N != 8 && N != 16 && N != 32 && N != 64) return MB200_ENSTATE;
   if (seqs->rows == 0 || ED == 0) return MB200_OK;
@@ -906,10 +909,10 @@ extern "C" int mb200_sscan_packed_fwd(const mb200_packed* seqs, const void* x, c
   p.B = 1; p.L = seqs->rows; p.ED = ED;
   p.x_sl = x_sl; p.d_sl = d_sl; p.z_sl = z_sl; p.b_sl = b_sl; p.c_sl = c_sl; p.y_sl = y_sl;
   p.flags = flags & (MB200_DELTA_SOFTPLUS | MB200_GENERAL_DECAY | MB200_PAIRED_STATES);
-  p.seqs = packed_of(*seqs, piece_len);
+  p.seqs = packed_of(*seqs, piece_len, parts);
   if (!states) p.seqs.slots = nullptr;
   p.pieceP = pieces;
-  p.pieceS = pieces ? pieces + packed_items(seqs->rows, seqs->sequences, piece_len) * ED * N : nullptr;
+  p.pieceS = pieces ? pieces + packed_items(seqs->rows, seqs->sequences, piece_len / parts) * ED * N : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int es = dtype == MB200_F32 ? 4 : 2;
   if (tma_path_ok(p, N, es)) {
@@ -917,7 +920,7 @@ extern "C" int mb200_sscan_packed_fwd(const mb200_packed* seqs, const void* x, c
     int rc = MB200_OK;
     if (piece_len) {
       SscanFwdParams c = p;
-      c.y = nullptr; c.z = nullptr; c.Cm = Bm; c.c_sl = b_sl; c.carries = nullptr;
+      c.y = nullptr; c.z = nullptr; c.Cm = Bm; c.c_sl = b_sl;
       rc = launch(c);
     }
     if (rc == MB200_OK) rc = launch(p);

@@ -146,6 +146,20 @@ def test_pieces(lengths, piece, W, dtype):
         close(a, b, a.dtype, "d" + k)
 
 
+@pytest.mark.parametrize("lengths", [[700, 33, 200, 0, 97, 1], [1000], [192, 193, 191], [97, 96, 95] * 3])
+@pytest.mark.parametrize("piece", [96, 192, 256])
+@pytest.mark.parametrize("W,dtype", [(32, torch.float32), (40, torch.bfloat16)])
+def test_pieces_in_parts(lengths, piece, W, dtype):
+    """Pieces long enough for their carries to come in 2 to 4 parts."""
+    test_pieces(lengths, piece, W, dtype)
+
+
+def test_many_cut_sequences():
+    """More sequences than a CTA has threads, some of them cut."""
+    lengths = [3, 0, 1, 40, 2] * 80 + [130, 1, 70]
+    test_pieces(lengths, 32, 32, torch.float32)
+
+
 @pytest.mark.parametrize("piece", [0, 16])
 def test_nothing_crosses_a_border(piece):
     """A sequence of NaN and infinities, and garbage behind the last one, leave the others as they are, bit for bit."""
