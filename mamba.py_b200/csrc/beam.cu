@@ -285,7 +285,8 @@ beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slic
 // ranks at a time as the threads can take; once a whole rank holds nothing ahead of the num-th highest so far, no further one does.  What
 // the argument above on lanes and warps does not rule out goes side by side in shared memory, where each counts those ahead of it.
 // Bound by latency: two round trips to global memory, a logarithm in 64 bits, and three or four barriers for every set of ranks (one or two sets in
-// general).  16 groups of 16 beams of 128256, 32 of them: 61 us with all 1024 candidates of a group in any order.
+// general).  16 groups of 16 beams of 128256, 32 of them: the join is 12 us of 57 (the slices' kernel 45), where it was 61 with all 1024 candidates
+// of a group in any order.
 __global__ void __launch_bounds__(kSelThreads)
 beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ best, const float* __restrict__ scores,
                  const uint8_t* __restrict__ finished, const void* __restrict__ logits, int64_t stride, int dtype, int beams, int n_slices, int V,
@@ -304,8 +305,10 @@ beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ 
   // Lists of the group, and how a set of candidates is made of them: whole ranks of all lists, or a part of one.
   const int lists = beams * n_slices, ranks = lists <= kSelThreads ? kSelThreads / lists : 1, parts = (lists + kSelThreads - 1) / kSelThreads;
   const int sets = parts > 1 ? num * parts : (num + ranks - 1) / ranks;
-  auto list_of = [&](int set) { return parts > 1 ? set % parts * kSelThreads + tid : tid < ranks * lists ? tid % lists : lists; };
-  auto rank_of = [&](int set) { return parts > 1 ? set / parts : set * ranks + tid / lists; };
+  // (a list's ranks side by side, so that every warp has some of the first ones)
+  const int my_list = tid / ranks, my_rank = tid % ranks;
+  auto list_of = [&](int set) { return parts > 1 ? set % parts * kSelThreads + tid : my_list; };
+  auto rank_of = [&](int set) { return parts > 1 ? set / parts : set * ranks + my_rank; };
   const uint64_t* const mine = best + g * lists * num;
   auto fetch = [&](int set) -> uint64_t {
     const int l = list_of(set), r = rank_of(set);
@@ -366,9 +369,11 @@ beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ 
   for (bool again = false;; again = true) {
     uint64_t least_order = 0, least_place = 0;             // of the num-th highest so far
     bool fresh = false;                                    // something of this rank went into the list
+    uint64_t first_order = 0, first_place = 0;             // the thread's candidate of the first set
     for (int set = 0; set < sets; ++set) {
       uint64_t place = 0;
       const uint64_t order = candidate(set, place);
+      if (set == 0) first_order = order, first_place = place;
       const uint32_t high = uint32_t(order >> 32);
       const uint32_t sorted = sorted_in_warp(high, lane);
       if (lane == (num <= 32 ? num : 32) - 1) s_least[0][warp] = num <= 32 ? sorted : 0;
@@ -380,8 +385,13 @@ beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ 
         most = max(most, s_least[0][w]);
         all = min(all, s_least[1][w]);
       }
-      if (order && high >= max(most, all) && (order > least_order || (order == least_order && place < least_place))) {
-        const int n = atomicAdd(&s_n, 1);
+      const bool in = order && high >= max(most, all) && (order > least_order || (order == least_order && place < least_place));
+      const unsigned who = __ballot_sync(0xffffffffu, in);
+      int base = 0;
+      if (lane == 0 && who) base = atomicAdd(&s_n, __popc(who));
+      base = __shfl_sync(0xffffffffu, base, 0);
+      if (in) {
+        const int n = base + __popc(who & ((1u << lane) - 1));
         s_order[n] = order;
         s_place[n] = place;
       }
@@ -389,15 +399,19 @@ beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ 
       const int n = s_n, kept = least_order ? num : 0;
       fresh = (parts > 1 && set % parts != 0 && fresh) || n > kept || !least_order;
       if (n > kept) {
-        for (int i = tid; i < n; i += kSelThreads) {
-          const uint64_t o = s_order[i], q = s_place[i];
+        // the lanes of a group of 8 count their eighths of what is ahead of a candidate (one thread a candidate: 62 candidates take 4 us)
+        for (int first = 0; first < n; first += kSelThreads / 8) {
+          const int i = first + tid / 8;
+          const uint64_t o = i < n ? s_order[i] : 0, q = i < n ? s_place[i] : 0;
           int ahead = 0;
 #pragma unroll 4
-          for (int k = 0; k < n; ++k) {
-            const uint64_t other = s_order[k];
-            ahead += other > o || (other == o && s_place[k] < q);
+          for (int k = tid % 8; k < n; k += 8) {
+            const uint64_t other = s_order[k], where = s_place[k];
+            ahead += int(other > o) | (int(other == o) & int(where < q));
           }
-          if (ahead < num) {
+#pragma unroll
+          for (int s = 4; s >= 1; s >>= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, s);
+          if (i < n && tid % 8 == 0 && ahead < num) {
             s_best[0][ahead] = o;
             s_best[1][ahead] = q;
           }
@@ -418,25 +432,28 @@ beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ 
       if (!fresh && (parts == 1 || set % parts == parts - 1)) break;
     }
     if (again) break;
-    // whether a candidate of another beam is too close to one that is chosen for 32 bits to tell them apart
+    // Whether 32 bits cannot tell candidates of different beams apart.  Neighbours among the chosen, and the last of them with those behind it,
+    // say it of all: between two that are too close, each is too close to the next.
     bool close = false;
-    const double apart = too_close(V), edge = value_of(s_best[0][num - 1]) - apart;
+    const double apart = too_close(V), last = value_of(s_best[0][num - 1]);
+    const int last_beam = int(s_best[1][num - 1] >> 32);
+    auto compare = [&](int k, int other) {
+      if (k == other || (s_kind[k] != kOpen && s_kind[other] != kOpen)) return;
+      close = true;
+      atomicOr(&s_close[k / 32], 1u << k % 32);
+      atomicOr(&s_close[other / 32], 1u << other % 32);
+    };
+    if (tid < num - 1) {
+      const double value = value_of(s_best[0][tid + 1]);
+      if (value > -INFINITY && value_of(s_best[0][tid]) - value <= apart) compare(int(s_best[1][tid] >> 32), int(s_best[1][tid + 1] >> 32));
+    }
     for (int set = 0; set < sets; ++set) {
-      uint64_t place = 0;
-      const uint64_t order = candidate(set, place);
+      uint64_t place = first_place;
+      const uint64_t order = set == 0 ? first_order : candidate(set, place);
       const double value = value_of(order);
-      const bool near = order && value > -INFINITY && value >= edge;
-      if (near) {
-        const int k = int(place >> 32);
-        for (int r = 0; r < num; ++r) {
-          const int other = int(s_best[1][r] >> 32);
-          if (fabs(value_of(s_best[0][r]) - value) > apart || other == k || (s_kind[other] != kOpen && s_kind[k] != kOpen)) continue;
-          close = true;
-          atomicOr(&s_close[k / 32], 1u << k % 32);
-          atomicOr(&s_close[other / 32], 1u << other % 32);
-        }
-      }
-      if (parts == 1 && !__syncthreads_or(near)) break;
+      const bool near = order && value > -INFINITY && last - value <= apart;
+      if (near && (order < least_order || (order == least_order && place > least_place))) compare(int(place >> 32), last_beam);
+      if (parts == 1 && (set + 1 == sets || !__syncthreads_or(near))) break;
     }
     if (!__syncthreads_or(close)) break;
     for (int k = 0; k < beams; ++k) {
@@ -478,7 +495,7 @@ beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ 
 //
 // Every CTA makes the list of copies for itself in shared memory (a launch and a round trip through global memory less), then takes its share of
 // (copy, part of a state) pairs.  Bound by HBM: each copied byte is read and written once.
-constexpr int kReorderThreads = 256, kReorderPart = 16384;  // bytes a CTA copies at a time
+constexpr int kReorderThreads = 256, kReorderPart = 8192;   // bytes a CTA copies at a time: 64 layers, 24 states of 328 KB, us with 4 / 8 / 16 / 32 / 64 KB 250 / 190 / 194 / 196 / 197
 constexpr int kMostSlotBeams = 4096, kMostPools = 128;
 
 struct Pools {
