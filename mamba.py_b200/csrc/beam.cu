@@ -71,10 +71,10 @@ __device__ __forceinline__ uint32_t sorted_in_warp(uint32_t x, int lane) {
 // every item counts those ahead of it; between chunks the num-th of them becomes the new K.  That may be a
 // value that very many logits share (a mask's): equal to K, then, counts only up to the num-th place that does, of which there are num in the
 // first chunk or none.  Should a chunk have more than there is room for all the same (ascending logits may), num rounds over the slice find the highest.
-// Bound: 8 instructions a logit (load and conversion, maximum, difference, product, ex2, sum), which is near the time that its 2 bytes take
+// Bound: 6 instructions a logit (load and conversion, maximum, half of a difference, product and sum, ex2), which is near the time that its 2 bytes take
 // from HBM, and some 2 us a CTA for the first chunk's sort and the counts at the end.  So a CTA takes as many chunks as leave
 // four CTAs for every SM, with the next chunk's loads in flight.  64 x 4 x 50280 in bfloat16: 58 us with a CTA to every 8192 logits and a count of
-// all threads' highest, 25 with the warps' sort, 22 with several chunks a CTA.
+// all threads' highest, 25 with the warps' sort, 22 with several chunks a CTA, 18 with the join's work and the exponentials' in pairs.
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kSelThreads, 4)
 beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slice, int num, Slice* __restrict__ slices, uint64_t* __restrict__ best) {
@@ -202,13 +202,14 @@ beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slic
       mine = top;
     }
     const float from = top == -INFINITY ? 0.f : top;
-    float sum4[4];
+    float2 sums[2];
 #pragma unroll
-    for (int j = 0; j < kSelPer; ++j) {
-      const float x = ex2f((v[j] - from) * kLog2e);
-      sum4[j % 4] = j < 4 ? x : sum4[j % 4] + x;
+    for (int j = 0; j < kSelPer; j += 2) {
+      const float2 t = __fmul2_rn(__fadd2_rn(make_float2(v[j], v[j + 1]), make_float2(-from, -from)), make_float2(kLog2e, kLog2e));
+      const float2 x = make_float2(ex2f(t.x), ex2f(t.y));
+      sums[j / 2 % 2] = j < 4 ? x : __fadd2_rn(sums[j / 2 % 2], x);
     }
-    all += double((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+    all += double((sums[0].x + sums[0].y) + (sums[1].x + sums[1].y));
     // Few threads look at their logits one by one, and read those that count again: a body for each of the 16 would cost more than all the rest.
     if (fmaxf(high, high2) >= least) {
       unsigned hits = 0;
@@ -285,7 +286,7 @@ beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slic
 // ranks at a time as the threads can take; once a whole rank holds nothing ahead of the num-th highest so far, no further one does.  What
 // the argument above on lanes and warps does not rule out goes side by side in shared memory, where each counts those ahead of it.
 // Bound by latency: two round trips to global memory, a logarithm in 64 bits, and three or four barriers for every set of ranks (one or two sets in
-// general).  16 groups of 16 beams of 128256, 32 of them: the join is 12 us of 57 (the slices' kernel 45), where it was 61 with all 1024 candidates
+// general).  16 groups of 16 beams of 128256, 32 of them: the join is 12 us of 55 (the slices' kernel 43), where it was 61 with all 1024 candidates
 // of a group in any order.
 __global__ void __launch_bounds__(kSelThreads)
 beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ best, const float* __restrict__ scores,
