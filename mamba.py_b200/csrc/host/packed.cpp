@@ -250,6 +250,7 @@ static Cut pick_cut(int64_t rows, int64_t sequences, int64_t longest, int64_t wi
     }
     const int64_t parts = parts_of(P, whole, tiles, sms);
     if (piece > 0) return {P, parts};
+    if (S > 1 && mb200_packed_parts(rows, sequences, P / parts) > 65535) break;      // more than a launch has room for
     main[0] = Group{double(P), whole};
     carry[0] = Group{double(P) / double(parts), whole * double(parts)};
     double us = pass(main, grad ? kFwdSaving : kFwd) + (grad ? pass(main, kBwd) : 0);
