@@ -98,6 +98,7 @@ struct PackedScanBackward : public torch::autograd::Node {
   at::ScalarType types[kInputs];
   bool given[kInputs];
   int64_t piece_len = 0, parts = 1;
+  std::vector<int64_t> D_shape, bias_shape;
 
   std::string name() const override { return "PackedSelectiveScanBackward"; }
   void release_variables() override {
@@ -121,7 +122,8 @@ struct PackedScanBackward : public torch::autograd::Node {
     const Tensor acc = empty({2 * T * N + W * N + 2 * W}, at::kFloat, a.x);
     zero_fill(acc);
     const Tensor dB = alias(acc, 0, {T, N}), dC = alias(acc, T * N, {T, N}), dA = alias(acc, 2 * T * N, {W, N}),
-                 dD = alias(acc, 2 * T * N + W * N, {W}), db = a.bias.defined() ? alias(acc, 2 * T * N + W * N + W, {W}) : Tensor();
+                 dD = alias(acc, 2 * T * N + W * N, given[kD] ? D_shape : std::vector<int64_t>{W}),
+                 db = a.bias.defined() ? alias(acc, 2 * T * N + W * N + W, bias_shape) : Tensor();
     const Tensor pg = piece_len ? empty({a.n_parts(), W, N}, at::kFloat, a.x) : Tensor(), car = carries.get(), pcs = pieces.get();
     const mb200_packed s = a.seqs.abi();
     check(mb200_sscan_packed_bwd(&s, ptr(a.x), ptr(a.delta), ptr(a.z), fptr(a.A), ptr(a.B), ptr(a.C), fptr(a.D), fptr(a.bias), ptr(dy), fptr(car),
@@ -150,7 +152,7 @@ Tensor filter(const Tensor& weight, int64_t width) {
 struct PackedConvBackward : public torch::autograd::Node {
   Saved x, w, b, cu;
   at::ScalarType tx, tw, tb;
-  std::vector<int64_t> w_shape;
+  std::vector<int64_t> w_shape, b_shape;
   std::string name() const override { return "PackedCausalConv1dSiluBackward"; }
   void release_variables() override {
     for (Saved* s : {&x, &w, &b, &cu}) s->reset();
@@ -165,7 +167,7 @@ struct PackedConvBackward : public torch::autograd::Node {
     const int64_t T = xs.size(0), W = xs.size(1), K = w32.size(1);
     const Tensor dx = empty({T, W}, xs.scalar_type(), xs), acc = empty({W * K + W}, at::kFloat, xs);
     zero_fill(acc);
-    const Tensor dw = alias(acc, 0, w_shape), db = b32.defined() ? alias(acc, W * K, {W}) : Tensor();
+    const Tensor dw = alias(acc, 0, w_shape), db = b32.defined() ? alias(acc, W * K, b_shape) : Tensor();
     Sequences q;
     q.cu = cu.get();
     q.rows = T;
@@ -325,6 +327,8 @@ Tensor selective_scan_packed(const Tensor& x, const Tensor& delta, const Tensor&
     node->x.save(a.x); node->delta.save(a.delta); node->A.save(a.A); node->B.save(a.B); node->C.save(a.C); node->D.save(a.D);
     node->z.save(a.z); node->bias.save(a.bias); node->cu.save(a.seqs.cu); node->carries.save(carries); node->pieces.save(pieces);
     node->piece_len = a.piece_len; node->parts = a.parts;
+    if (D.defined()) node->D_shape = D.sizes().vec();
+    if (bias.defined()) node->bias_shape = bias.sizes().vec();
     torch::autograd::set_history(y, node);
   }
   return y;
@@ -368,6 +372,7 @@ Tensor conv1d_silu_packed(const Tensor& x, const Tensor& weight, const OptTensor
     node->x.save(xs); node->w.save(w32); node->b.save(b32); node->cu.save(q.cu);
     node->tx = type_of(x); node->tw = type_of(weight); node->tb = type_of(bias);
     node->w_shape = weight.sizes().vec();
+    if (bias.defined()) node->b_shape = bias.sizes().vec();
     torch::autograd::set_history(y, node);
   }
   return y;

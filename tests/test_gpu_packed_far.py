@@ -129,7 +129,9 @@ def test_broadcast_and_strided_inputs(W):
     cu = cu_of(lengths, torch.int64)
     odd = dict(t, x=t["x"].t().contiguous().t(), delta=t["delta"][:1].expand(T, W), B=torch.stack([t["B"], t["C"]], 1).view(2 * T, 16)[::2],
                z=t["z"][:, :1].expand(T, W))
+    odd["D"], odd["delta_bias"] = t["D"].view(1, W), t["delta_bias"].view(W, 1)
     same = {k: v.contiguous() for k, v in odd.items()}
+    same["D"], same["delta_bias"] = t["D"], t["delta_bias"]
     runs = []
     for q in (odd, same):
         leaves = {k: v.detach().requires_grad_() for k, v in q.items()}
@@ -137,13 +139,14 @@ def test_broadcast_and_strided_inputs(W):
         runs.append((y, torch.autograd.grad(y.sum(), list(leaves.values()))))
     close(runs[0][0], runs[1][0], what="y")
     for k, a, b in zip(odd, runs[0][1], runs[1][1]):
-        close(a, b, what=k)
-    weight = torch.randn(W, 1, 4, device=DEV, requires_grad=True)
+        assert a.shape == odd[k].shape
+        close(a.reshape(b.shape), b, what=k)
+    weight, bias = torch.randn(W, 1, 4, device=DEV, requires_grad=True), torch.randn(1, W, device=DEV, requires_grad=True)
     runs = []
     for x in (odd["x"], same["x"], t["x"][:1].expand(T, W), t["x"][:1].repeat(T, 1)):
         leaf = x.detach().requires_grad_()
-        y = mamba_b200.causal_conv1d_silu_packed(leaf, weight, cu_seqlens=cu)
-        runs.append((y, *torch.autograd.grad(y.sum(), (leaf, weight))))
+        y = mamba_b200.causal_conv1d_silu_packed(leaf, weight, bias, cu_seqlens=cu)
+        runs.append((y, *torch.autograd.grad(y.sum(), (leaf, weight, bias))))
     for a, b in (runs[:2], runs[2:]):
         for u, v in zip(a, b):
             close(u, v)
@@ -159,3 +162,23 @@ def test_the_last_choice_of_a_large_vocabulary():
     got = mamba_b200.beam_select(logits, scores)
     want = mamba_b200.beam_select(logits[-2:].clone(), scores[-2:].clone())
     assert torch.equal(got[0][-2:], want[0]) and torch.equal(got[1][-2:], want[1]) and torch.equal(got[2][-2:], want[2])
+
+
+@pytest.mark.parametrize("piece", [0, 32])
+def test_backward_twice_and_mixed_types(piece):
+    """One forward, two backward passes; activations and parameters of different types get gradients of their own."""
+    import mamba_b200
+    lengths = [100, 0, 37]
+    t = inputs(11, sum(lengths), 64, dtype=torch.bfloat16)
+    t["z"], t["A"], t["D"] = t["z"].float(), t["A"].bfloat16(), t["D"].bfloat16()
+    leaves = {k: v.requires_grad_() for k, v in t.items()}
+    y = mamba_b200.selective_scan_packed(**leaves, cu_seqlens=cu_of(lengths), piece_length=piece)
+    dy = torch.randn_like(y)
+    first = torch.autograd.grad(y, list(leaves.values()), dy, retain_graph=True)
+    second = torch.autograd.grad(y, list(leaves.values()), dy)
+    wide = {k: v.detach().float().requires_grad_() for k, v in t.items()}
+    want = torch.autograd.grad(mamba_b200.selective_scan_packed(**wide, cu_seqlens=cu_of(lengths), piece_length=piece), list(wide.values()), dy.float())
+    for (k, v), a, b, w in zip(leaves.items(), first, second, want):
+        assert a.dtype == b.dtype == v.dtype and a.shape == v.shape
+        close(a, w, v.dtype, what=k)
+        one_step(a, b) if v.dtype == torch.bfloat16 else close(a, b, what=k)
