@@ -56,8 +56,10 @@ ssm_step_kernel(const T* __restrict__ x, const T* __restrict__ delta, const T* _
   const int tid = threadIdx.x;
   const int q = tid % kLPE;
   const int64_t e = int64_t(blockIdx.x) * kEPB + tid / kLPE;
-  const int64_t b = blockIdx.y, hb = kSlots ? __ldg(slots + b) : b;
-  const bool mine = e < ED, ok = mine && (!kSlots || (hb >= 0 && hb < n_slots));
+  const bool mine = e < ED;
+  const int64_t b = blockIdx.y;
+  int64_t hb = b; bool ok = mine;
+  if constexpr (kSlots) { hb = __ldg(slots + b); ok = mine && hb >= 0 && hb < n_slots; }
   float yv = 0.f, xv = 0.f, zv = 0.f;
   if (ok) {
     // the state is the only large stream: get it moving first, everything else is small
