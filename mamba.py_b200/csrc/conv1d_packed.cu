@@ -406,14 +406,33 @@ conv1d_silu_packed_tma_kernel(const __grid_constant__ CUtensorMap map, const Pac
 // dx[t] = sum_j w[3-j] * dpre[t+j] over the rows t+j of t's sequence;  dw[k] = sum_t dpre[t] * in(t-3+k);  dbias = sum dpre;
 // dpre[t] = dy[t] * silu'(pre[t]), pre recomputed from x.  Sequences that resume have no backward, so in = 0 before a first row.
 // As on rectangles the windows hold as many rows as a group, dx trails by three rows, and the 4 warps of a CTA add their sums in shared memory.
+// With four channels a thread, rows come through a ring in shared memory, groups ahead of the arithmetic: each thread copies what it
+// reads itself, so its own waits are all it takes, and no register holds what is on its way.  16000 x 1536: float32 70 -> 58 us (HBM at 4.9 TB/s,
+// the shared-memory pipe next; 68 with copies that go through L1), bfloat16 51 -> 40 (half of the issue slots, with 13 warps an SM).
 constexpr int kPkBwdThreads = 128, kPkBwdWarps = kPkBwdThreads / 32, kPkBwdChunkMost = 128;
+
+template <typename T> constexpr int kPkBwdStages = sizeof(T) == 2 ? 4 : 3;      // groups of four rows of x and dy
+template <typename T, int V> constexpr int kPkBwdRing = V == 1 ? 0 : kPkBwdThreads * kPkBwdStages<T> * 2 * kConvK * int(sizeof(T)) * V;
+
+// This thread's copy of kBytes to shared memory; zeros if not `ok`.
+template <int kBytes>
+__device__ __forceinline__ void copy_ahead(void* to, const void* from, const void* valid, bool ok) {
+  const unsigned at = unsigned(__cvta_generic_to_shared(to));
+  const int n = ok ? kBytes : 0;
+  if constexpr (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(ok ? from : valid), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(at), "l"(ok ? from : valid), "n"(kBytes), "r"(n) : "memory");
+}
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kPkBwdThreads, 4)
 conv1d_silu_packed_bwd_kernel(const Packed seqs, const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ bias,
                               const T* __restrict__ dy, T* __restrict__ dx, float* __restrict__ dw, float* __restrict__ dbias, int64_t ED,
                               int64_t x_sl, int64_t dy_sl, int64_t dx_sl, int chunk) {
-  constexpr int kG = kConvK, kH = kConvK - 1;
+  constexpr int kG = kConvK, kH = kConvK - 1, kStages = kPkBwdStages<T>;
+  constexpr bool kRing = V > 1;
+  extern __shared__ __align__(16) unsigned char ring[];
   constexpr int kBits = kH + kPkBwdWarps * kPkBwdChunkMost + kH;
   __shared__ float s_acc[32 * V * (kConvK + 1)];          // per channel of the CTA: dw[0..3], dbias
   __shared__ unsigned s_first[(kBits + 31) / 32 + 1];     // bit i: a sequence begins at row T0 - 3 + i
@@ -466,14 +485,32 @@ conv1d_silu_packed_bwd_kernel(const Packed seqs, const T* __restrict__ x, const 
     }
     const F one = F::splat(1.f), mone = F::splat(-1.f), zero = F::splat(0.f);
     const int own = t1 - t0, end = min(tail, t1 + kH) - t0;
+    CVec<T, V>* const mine = reinterpret_cast<CVec<T, V>*>(ring) + warp * (kStages * 2 * kG * 32) + lane;
+    int stage = 0;
+    auto ahead = [&](int s0, int to) {
+      if (s0 < own + kH) {
+#pragma unroll
+        for (int j = 0; j < kG; ++j) {
+          copy_ahead<sizeof(T) * V>(mine + (to * 2 * kG + j) * 32, xg, x, s0 + j < end);
+          copy_ahead<sizeof(T) * V>(mine + (to * 2 * kG + kG + j) * 32, gg, x, s0 + j < end);
+          xg += x_sl; gg += dy_sl;
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
     auto group = [&](auto plain, int s0, unsigned f) {    // f: bits of rows s0 - 3 .. s0 + 3; plain: inside the chunk, and none set
       constexpr bool kPlain = decltype(plain)::value;
       CVec<T, V> qx[kG], qg[kG];
 #pragma unroll
       for (int j = 0; j < kG; ++j) {
-        qx[j] = cload<T, V>(xg, kPlain || s0 + j < end);
-        qg[j] = cload<T, V>(gg, kPlain || s0 + j < end);
-        xg += x_sl; gg += dy_sl;
+        if constexpr (kRing) {
+          qx[j] = mine[(stage * 2 * kG + j) * 32];
+          qg[j] = mine[(stage * 2 * kG + kG + j) * 32];
+        } else {
+          qx[j] = cload<T, V>(xg, kPlain || s0 + j < end);
+          qg[j] = cload<T, V>(gg, kPlain || s0 + j < end);
+          xg += x_sl; gg += dy_sl;
+        }
       }
 #pragma unroll
       for (int j = 0; j < kG; ++j) {
@@ -512,11 +549,20 @@ conv1d_silu_packed_bwd_kernel(const Packed seqs, const T* __restrict__ x, const 
         og += dx_sl;
       }
     };
+    if constexpr (kRing) {
+#pragma unroll
+      for (int i = 0; i < kStages - 1; ++i) ahead(i * kG, i);
+    }
 #pragma unroll 1
     for (int s0 = 0; s0 < own + kH; s0 += kG) {
+      if constexpr (kRing) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        ahead(s0 + (kStages - 1) * kG, stage == 0 ? kStages - 1 : stage - 1);
+      }
       const unsigned f = firsts_at(t0 + s0);
       if (f == 0 && s0 >= kH && s0 + kG <= own && s0 + kG <= end) group(std::true_type{}, s0, f);
       else group(std::false_type{}, s0, f);
+      if (kRing && ++stage == kStages) stage = 0;
     }
 #pragma unroll
     for (int i = 0; i < P; ++i) {
@@ -560,8 +606,8 @@ int packed_chunk(int64_t rows, int64_t cols, int warps, int resident, int unit, 
 
 // Channels of a thread of the backward.  Four save instructions, one gives four times the warps: us with four / one, with the launches around it,
 //            1000 x 512   3000 x 1000   8000 x 512   4000 x 1536   2000 x 5120   8000 x 1536   16000 x 1536
-// float32     8.0 / 5.7    13.1 / 10.9    14.9 / 14.4  24.2 / 27.4   37.4 / 47.5   43.8 / 54.7   70.2 / 94.5
-// bfloat16    7.7 / 5.8    12.5 / 11.1    15.2 / 12.3  17.3 / 16.2   26.0 / 36.8   30.4 / 47.3   51.0 / 87.1
+// float32     7.5 / 5.9    12.5 / 10.2    14.9 / 13.0  18.7 / 25.8   29.5 / 44.2   35.9 / 53.2   58.2 / 90.1
+// bfloat16    7.2 / 5.5    12.7 / 11.0    15.0 / 11.9  18.2 / 16.2   23.9 / 34.5   26.8 / 45.6   40.0 / 86.4
 bool one_channel(int64_t values, int dtype) { return values <= (dtype == MB200_F32 ? int64_t(9) << 19 : int64_t(7) << 20); }
 
 int check_conv(const mb200_packed* seqs, int64_t ED, int K, int dtype) {
@@ -630,10 +676,15 @@ extern "C" int mb200_conv1d_silu_packed_bwd(const mb200_packed* seqs, const void
   const int chunk = packed_chunk(seqs->rows, cols, kPkBwdWarps, 4, 8, kPkBwdChunkMost, 16);
   const dim3 grid(unsigned((seqs->rows + kPkBwdWarps * chunk - 1) / (kPkBwdWarps * chunk)), unsigned(cols));
   const Packed k = packed_of(*seqs, 0);
-#define MB200_CONV_BWD(TT, VV) \
-  conv1d_silu_packed_bwd_kernel<TT, VV><<<grid, kPkBwdThreads, 0, st>>>(k, (const TT*)x, w, bias, (const TT*)dy, (TT*)dx, dw, dbias, ED, x_sl, dy_sl, dx_sl, chunk)
-  if (dtype == MB200_F32) { if (vec) MB200_CONV_BWD(float, 4); else MB200_CONV_BWD(float, 1); }
-  else { if (vec) MB200_CONV_BWD(__nv_bfloat16, 4); else MB200_CONV_BWD(__nv_bfloat16, 1); }
+#define MB200_CONV_BWD(TT, VV)                                                                                                                  \
+  {                                                                                                                                             \
+    auto* const kernel = conv1d_silu_packed_bwd_kernel<TT, VV>;                                                                                 \
+    constexpr int bytes = kPkBwdRing<TT, VV>;                                                                                                   \
+    if (bytes && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return MB200_ELAUNCH;         \
+    kernel<<<grid, kPkBwdThreads, bytes, st>>>(k, (const TT*)x, w, bias, (const TT*)dy, (TT*)dx, dw, dbias, ED, x_sl, dy_sl, dx_sl, chunk);     \
+  }
+  if (dtype == MB200_F32) { if (vec) MB200_CONV_BWD(float, 4) else MB200_CONV_BWD(float, 1) }
+  else { if (vec) MB200_CONV_BWD(__nv_bfloat16, 4) else MB200_CONV_BWD(__nv_bfloat16, 1) }
 #undef MB200_CONV_BWD
   return check_launch();
 }
