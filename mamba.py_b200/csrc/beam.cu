@@ -496,7 +496,8 @@ beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ 
 //
 // Every CTA makes the list of copies for itself in shared memory (a launch and a round trip through global memory less), then takes its share of
 // (copy, part of a state) pairs.  Bound by HBM: each copied byte is read and written once.
-constexpr int kReorderThreads = 256, kReorderPart = 8192;   // bytes a CTA copies at a time: 64 layers, 24 states of 328 KB, us with 4 / 8 / 16 / 32 / 64 KB 250 / 190 / 194 / 196 / 197
+constexpr int kReorderThreads = 256, kReorderPart = 8192;
+// (bytes a CTA copies at a time: 64 layers, 24 states of 328 KB, us with 4 / 8 / 16 / 32 / 64 KB 250 / 190 / 194 / 196 / 197)
 constexpr int kMostSlotBeams = 4096, kMostPools = 128;
 
 struct Pools {

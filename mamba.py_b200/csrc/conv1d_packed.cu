@@ -83,8 +83,8 @@ __device__ __forceinline__ void leave_window(const Packed& seqs, int r, int t, b
 
 // The thread that meets a sequence's first row also leaves the window, when it is done with its rows: the only one that reads what the slot held.  So
 // the (at most two) rows after a first row that need it too, when they fall into the next chunk, are done by the chunk of the first row.
-// This form takes any strides, with one channel a thread; the tensor-map form below takes the others.  A warp finds out by itself which sequences begin in its rows, a lane a sequence, while the first rows and the filter are on their way: no
-// barrier, and for up to 32 sequences one load.
+// This form takes any strides, with one channel a thread; the tensor-map form below takes the others.  A warp finds out by itself which sequences
+// begin in its rows, a lane a sequence, while the first rows and the filter are on their way: no barrier, and for up to 32 sequences one load.
 template <typename T>
 __global__ void __launch_bounds__(kPkThreads, kPkResident)
 conv1d_silu_packed_fwd_kernel(const Packed seqs, const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ bias,
@@ -256,7 +256,8 @@ __global__ void __launch_bounds__(kTcThreads, kTcResident)
 conv1d_silu_packed_tma_kernel(const __grid_constant__ CUtensorMap map, const Packed seqs, const T* __restrict__ x,
                               const float* __restrict__ w, const float* __restrict__ bias, T* __restrict__ y, T* windows,
                               int64_t ED, int64_t x_sl, int64_t y_sl) {
-  constexpr int kTcChannels = kTcBytes / int(sizeof(T)), V = kTcChannels / 32, W = 2, P = V / W, kMine = kTcRows / kTcWarps, kBefore = kConvK - 2, kSeen = kBefore + kTcRows + kConvK - 2;
+  constexpr int kTcChannels = kTcBytes / int(sizeof(T)), V = kTcChannels / 32, W = 2, P = V / W;
+  constexpr int kMine = kTcRows / kTcWarps, kBefore = kConvK - 2, kSeen = kBefore + kTcRows + kConvK - 2;
   constexpr int kBytes = kTcBox * kTcBytes;
   static_assert(kBytes % 128 == 0, "boxes stay aligned");
   struct Begins { int64_t slot; int seq; bool old; };     // a sequence, its slot or -1, and whether it resumes

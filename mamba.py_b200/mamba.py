@@ -111,7 +111,8 @@ def causal_conv1d_silu(x, weight, bias=None):
 
 
 def causal_conv1d_silu_packed(x, weight, bias=None, *, cu_seqlens, windows=None, slots=None, resume=None):
-    """`causal_conv1d_silu` over sequences of different lengths laid end to end: x (T, ED), cu_seqlens as for `selective_scan_packed`.
+    """`causal_conv1d_silu` (d_conv 4) over sequences of different lengths laid end to end: x (T, ED), cu_seqlens as for
+    `selective_scan_packed`.
 
     With gradients for training; for serving `windows` (S, ED, 3), of x's dtype, is a pool whose entry slots[r] sequence r leaves its last
     three inputs in, and starts from where `resume` says so."""
