@@ -142,6 +142,16 @@ def test_select_where_beams_are_alike():
     check_select((base + torch.randn(4, 5, 1, generator=g)).to(DEV), -torch.rand(4, 1, generator=g).repeat(1, 5).to(DEV), 40)
 
 
+@pytest.mark.parametrize("K,V,num", [(64, 50280, 64), (40, 60000, 10), (64, 30000, 1), (33, 40000, 33)])
+def test_select_of_more_slices_than_threads(K, V, num):
+    """One group whose beams' slices are more than the joining CTA has threads; the second time with beams that only 64 bits tell apart."""
+    g = torch.Generator().manual_seed(K)
+    check_select(torch.randn(1, K, V, generator=g).to(DEV), -torch.rand(1, K, generator=g).to(DEV), num)
+    alike = torch.randn(1, 1, V, generator=g) + torch.randn(1, K, 1, generator=g)
+    check_select(alike.to(DEV), torch.zeros(1, K, device=DEV), num)
+    check_select(alike.to(DEV).bfloat16(), torch.zeros(1, K, device=DEV), num, (torch.rand(1, K, generator=g) < 0.3).to(DEV), V - 1)
+
+
 def test_select_strides_and_order():
     """Ascending logits (every thread's highest is its last), descending ones, views with other strides, an offset of one element."""
     g = torch.Generator().manual_seed(0)
