@@ -407,31 +407,29 @@ conv1d_silu_packed_tma_kernel(const __grid_constant__ CUtensorMap map, const Pac
 // dx[t] = sum_j w[3-j] * dpre[t+j] over the rows t+j of t's sequence;  dw[k] = sum_t dpre[t] * in(t-3+k);  dbias = sum dpre;
 // dpre[t] = dy[t] * silu'(pre[t]), pre recomputed from x.  Sequences that resume have no backward, so in = 0 before a first row.
 // As on rectangles the windows hold as many rows as a group, dx trails by three rows, and the 4 warps of a CTA add their sums in shared memory.
-// With four channels a thread, rows come through a ring in shared memory, groups ahead of the arithmetic: each thread copies what it
-// reads itself, so its own waits are all it takes, and no register holds what is on its way.  16000 x 1536: float32 70 -> 58 us (HBM at 4.9 TB/s,
-// the shared-memory pipe next; 68 with copies that go through L1), bfloat16 51 -> 40 (half of the issue slots, with 13 warps an SM).
+// Of large tensors a thread takes 8 bytes of channels, and rows come through a ring in shared memory, groups ahead of the arithmetic: each thread copies
+// what it reads itself, so its own waits are all it takes, and no register holds what is on its way.  16000 x 1536 without / with the ring: float32
+// 70 (four channels) / 52 us (two; four 57), bfloat16 51 / 40 (two channels: 45).  Four stages of the ring take the L1 that the copies pass through
+// (float32 62), two cost bfloat16 2 us.  Then bfloat16 waits for issue slots (half of them, with 13 warps an SM), float32 for HBM (5.6 TB/s).
 constexpr int kPkBwdThreads = 128, kPkBwdWarps = kPkBwdThreads / 32, kPkBwdChunkMost = 128;
-
-template <typename T> constexpr int kPkBwdStages = sizeof(T) == 2 ? 4 : 3;      // groups of four rows of x and dy
-template <typename T, int V> constexpr int kPkBwdRing = V == 1 ? 0 : kPkBwdThreads * kPkBwdStages<T> * 2 * kConvK * int(sizeof(T)) * V;
+constexpr int kPkBwdStages = 3;                          // groups of four rows of x and dy
+template <typename T, int V> constexpr int kPkBwdRing = V == 1 ? 0 : kPkBwdThreads * kPkBwdStages * 2 * kConvK * int(sizeof(T)) * V;
+template <int V> constexpr int kPkBwdResident = V == 2 ? 5 : 4;
 
 // This thread's copy of kBytes to shared memory; zeros if not `ok`.
 template <int kBytes>
 __device__ __forceinline__ void copy_ahead(void* to, const void* from, const void* valid, bool ok) {
   const unsigned at = unsigned(__cvta_generic_to_shared(to));
   const int n = ok ? kBytes : 0;
-  if constexpr (kBytes == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(ok ? from : valid), "r"(n) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(at), "l"(ok ? from : valid), "n"(kBytes), "r"(n) : "memory");
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(at), "l"(ok ? from : valid), "n"(kBytes), "r"(n) : "memory");
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kPkBwdThreads, 4)
+__global__ void __launch_bounds__(kPkBwdThreads, kPkBwdResident<V>)
 conv1d_silu_packed_bwd_kernel(const Packed seqs, const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ bias,
                               const T* __restrict__ dy, T* __restrict__ dx, float* __restrict__ dw, float* __restrict__ dbias, int64_t ED,
                               int64_t x_sl, int64_t dy_sl, int64_t dx_sl, int chunk) {
-  constexpr int kG = kConvK, kH = kConvK - 1, kStages = kPkBwdStages<T>;
+  constexpr int kG = kConvK, kH = kConvK - 1, kStages = kPkBwdStages;
   constexpr bool kRing = V > 1;
   extern __shared__ __align__(16) unsigned char ring[];
   constexpr int kBits = kH + kPkBwdWarps * kPkBwdChunkMost + kH;
@@ -605,10 +603,10 @@ int packed_chunk(int64_t rows, int64_t cols, int warps, int resident, int unit, 
   return best;
 }
 
-// Channels of a thread of the backward.  Four save instructions, one gives four times the warps: us with four / one, with the launches around it,
+// Channels of a thread of the backward: 8 bytes of them save instructions, one gives more warps.  us so / with one, with the launches around it:
 //            1000 x 512   3000 x 1000   8000 x 512   4000 x 1536   2000 x 5120   8000 x 1536   16000 x 1536
-// float32     7.5 / 5.9    12.5 / 10.2    14.9 / 13.0  18.7 / 25.8   29.5 / 44.2   35.9 / 53.2   58.2 / 90.1
-// bfloat16    7.2 / 5.5    12.7 / 11.0    15.0 / 11.9  18.2 / 16.2   23.9 / 34.5   26.8 / 45.6   40.0 / 86.4
+// float32     5.7 / 5.9    12.0 / 10.2    15.0 / 13.0  17.9 / 25.8   26.0 / 44.2   33.1 / 53.2   52.2 / 90.1
+// bfloat16    7.2 / 5.5    12.7 / 11.0    15.0 / 11.9  18.2 / 16.2   23.7 / 34.5   26.3 / 45.6   39.8 / 86.4
 bool one_channel(int64_t values, int dtype) { return values <= (dtype == MB200_F32 ? int64_t(9) << 19 : int64_t(7) << 20); }
 
 int check_conv(const mb200_packed* seqs, int64_t ED, int K, int dtype) {
@@ -670,11 +668,11 @@ extern "C" int mb200_conv1d_silu_packed_bwd(const mb200_packed* seqs, const void
   if (seqs->rows == 0 || ED == 0) return MB200_OK;
   if (!x || !w || !dy || !dx || !dw || seqs->slots) return MB200_EINVAL;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int kv = 4;
+  const int kv = dtype == MB200_F32 ? 2 : 4;
   const bool vec = !one_channel(seqs->rows * ED, dtype) && conv_vec_ok(ED, kv, {x, dy, (const void*)dx}, {x_sl, dy_sl, dx_sl});
   const int v = vec ? kv : 1;
   const int64_t cols = (ED + 32 * int64_t(v) - 1) / (32 * int64_t(v));
-  const int chunk = packed_chunk(seqs->rows, cols, kPkBwdWarps, 4, 8, kPkBwdChunkMost, 16);
+  const int chunk = packed_chunk(seqs->rows, cols, kPkBwdWarps, v == 2 ? kPkBwdResident<2> : kPkBwdResident<1>, 8, kPkBwdChunkMost, 16);
   const dim3 grid(unsigned((seqs->rows + kPkBwdWarps * chunk - 1) / (kPkBwdWarps * chunk)), unsigned(cols));
   const Packed k = packed_of(*seqs, 0);
 #define MB200_CONV_BWD(TT, VV)                                                                                                                  \
@@ -684,7 +682,7 @@ extern "C" int mb200_conv1d_silu_packed_bwd(const mb200_packed* seqs, const void
     if (bytes && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return MB200_ELAUNCH;         \
     kernel<<<grid, kPkBwdThreads, bytes, st>>>(k, (const TT*)x, w, bias, (const TT*)dy, (TT*)dx, dw, dbias, ED, x_sl, dy_sl, dx_sl, chunk);     \
   }
-  if (dtype == MB200_F32) { if (vec) MB200_CONV_BWD(float, 4) else MB200_CONV_BWD(float, 1) }
+  if (dtype == MB200_F32) { if (vec) MB200_CONV_BWD(float, 2) else MB200_CONV_BWD(float, 1) }
   else { if (vec) MB200_CONV_BWD(__nv_bfloat16, 4) else MB200_CONV_BWD(__nv_bfloat16, 1) }
 #undef MB200_CONV_BWD
   return check_launch();
