@@ -14,10 +14,8 @@ namespace {
 // The order is that of the values in 64 bits, at the price of 32: the logsumexp is off by a few 2^-20 (see too_close), and where candidates of
 // different beams come that close, which is a few groups in a hundred calls, the joining CTA sums those beams' exponentials again in 64 bits.
 
-constexpr int kSelThreads = 256, kSelWarps = kSelThreads / 32, kSelPer = 16;             // logits of a thread at a time
-constexpr int kSelChunk = kSelThreads * kSelPer;
+constexpr int kSelPer = 16;                                // logits of a thread at a time
 constexpr int kMostNum = 64, kMostBeams = 64;
-constexpr int kList = 1024;                                // items side by side in shared memory
 constexpr int kCheck = 4;                                  // chunks after which the list is looked at
 
 // By how much two logsumexps may be apart for rounding alone.  An exponent t = (v - top) log2(e) is off by 2.25 x 2^-24 |t| (a difference, a product,
@@ -65,7 +63,7 @@ __device__ __forceinline__ uint32_t sorted_in_warp(uint32_t x, int lane) {
   return x;
 }
 
-// How the highest are found.  A warp in which num lanes hold a value as high as K holds num that high, and so do the kSelWarps warps together if
+// How the highest are found.  A warp in which num lanes hold a value as high as K holds num that high, and so do the CTA's warps together if
 // each has its share of lanes that high; so no logit below K is wanted.  The higher of the two, over the slice's first chunk and the threads' own
 // highest, is K.  Whatever reaches K, in the chunks that follow too (about num a chunk, if they are alike), is put side by side with its place, and
 // every item counts those ahead of it; between chunks the num-th of them becomes the new K.  That may be a
@@ -73,15 +71,16 @@ __device__ __forceinline__ uint32_t sorted_in_warp(uint32_t x, int lane) {
 // first chunk or none.  Should a chunk have more than there is room for all the same (ascending logits may), num rounds over the slice find the highest.
 // Bound: 6 instructions a logit (load and conversion, maximum, half of a difference, product and sum, ex2), which is near the time that its 2 bytes take
 // from HBM, and some 2 us a CTA for the first chunk's sort and the counts at the end.  So a CTA takes as many chunks as leave
-// four CTAs for every SM, with the next chunk's loads in flight.  64 x 4 x 50280 in bfloat16: 58 us with a CTA to every 8192 logits and a count of
+// 1024 threads for every SM, with the next chunk's loads in flight.  64 x 4 x 50280 in bfloat16: 58 us with a CTA to every 8192 logits and a count of
 // all threads' highest, 25 with the warps' sort, 22 with several chunks a CTA, 18 with the join's work and the exponentials' in pairs.
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(kSelThreads, 4)
+template <typename T, bool kVec, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
 beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slice, int num, Slice* __restrict__ slices, uint64_t* __restrict__ best) {
-  __shared__ uint64_t s_list[kList], s_best[kMostNum], s_key[kSelWarps];
-  __shared__ uint32_t s_least[2][kSelWarps];
-  __shared__ float s_top[kSelWarps];
-  __shared__ double s_sum[kSelWarps];
+  constexpr int kWarps = kThreads / 32, kChunk = kThreads * kSelPer, kList = 4 * kThreads;      // kList: items side by side in shared memory
+  __shared__ uint64_t s_list[kList], s_best[kMostNum], s_key[kWarps];
+  __shared__ uint32_t s_least[2][kWarps];
+  __shared__ float s_top[kWarps];
+  __shared__ double s_sum[kWarps];
   __shared__ int s_n;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = blockIdx.y, part = row * gridDim.x + blockIdx.x;
@@ -91,8 +90,14 @@ beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slic
   cudaTriggerProgrammaticLaunchCompletion();               // the joining kernel may start, and waits for this one's end
   constexpr int kE = kVec ? Elem<T>::kVec : 1, kLoads = kSelPer / kE;
   struct alignas(sizeof(T) * kE) Raw { T v[kE]; };
-  auto at = [&](int c0, int j) { return c0 + ((j / kE) * kSelThreads + tid) * kE + j % kE; };
+  auto at = [&](int c0, int j) { return c0 + ((j / kE) * kThreads + tid) * kE + j % kE; };
   auto fetch = [&](int c0, Raw (&raw)[kLoads]) {
+    if (kVec && c0 + kChunk <= v1) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        if constexpr (kVec) *reinterpret_cast<uint4*>(&raw[i]) = __ldcs(reinterpret_cast<const uint4*>(p + at(c0, i * kE)));
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int c = at(c0, i * kE);
@@ -106,7 +111,7 @@ beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slic
   };
   // num highest of the list, highest first, in s_best
   auto rank = [&](int n) {
-    for (int i = tid; i < n; i += kSelThreads) {
+    for (int i = tid; i < n; i += kThreads) {
       const uint64_t key = s_list[i];
       int ahead = 0;
 #pragma unroll 4
@@ -122,7 +127,7 @@ beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slic
   float mine = -INFINITY;                                  // the thread's maximum,
   double all = 0.;                                         // and its sum of exp(logit - maximum)
   bool room = true;
-  for (int c0 = v0, chunk = 0; c0 < v1; c0 += kSelChunk, ++chunk) {
+  for (int c0 = v0, chunk = 0; c0 < v1; c0 += kChunk, ++chunk) {
     float v[kSelPer];
 #pragma unroll
     for (int j = 0; j < kSelPer; j += 2) {
@@ -133,7 +138,7 @@ beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slic
         v[j] = Elem<T>::to_f(raw[j].v[0]); v[j + 1] = Elem<T>::to_f(raw[j + 1].v[0]);
       }
     }
-    if (c0 + kSelChunk < v1) fetch(c0 + kSelChunk, raw);
+    if (c0 + kChunk < v1) fetch(c0 + kChunk, raw);
     float high = -INFINITY, high2 = -INFINITY;             // of the halves
 #pragma unroll
     for (int j = 0; j < kSelPer / 2; ++j) {
@@ -145,7 +150,7 @@ beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slic
       const uint32_t x = sorted_in_warp(order_of(fmaxf(high, high2)), lane);
       uint32_t whole = __shfl_sync(0xffffffffu, x, (num <= 32 ? num : 32) - 1);
       if (num > 32) whole = __reduce_min_sync(0xffffffffu, order_of(fminf(high, high2)));
-      const uint32_t share = __shfl_sync(0xffffffffu, x, (num + kSelWarps - 1) / kSelWarps - 1);
+      const uint32_t share = __shfl_sync(0xffffffffu, x, (num + kWarps - 1) / kWarps - 1);
       if (lane == 0) {
         s_least[0][warp] = whole;
         s_least[1][warp] = share;
@@ -153,7 +158,7 @@ beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slic
       __syncthreads();
       uint32_t most = 0, all = ~0u;
 #pragma unroll
-      for (int w = 0; w < kSelWarps; ++w) {
+      for (int w = 0; w < kWarps; ++w) {
         most = max(most, s_least[0][w]);
         all = min(all, s_least[1][w]);
       }
@@ -179,7 +184,7 @@ beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slic
           if (lane == 31) s_least[0][warp] = upto;
           __syncthreads();
           int total = 0;
-          for (int w = 0; w < kSelWarps; ++w) {
+          for (int w = 0; w < kWarps; ++w) {
             if (w < warp) upto += s_least[0][w];
             total += s_least[0][w];
           }
@@ -224,7 +229,7 @@ beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slic
         if (n < kList) s_list[n] = key_of(x, c);
       }
     }
-    if (c0 + kSelChunk >= v1) break;
+    if (c0 + kChunk >= v1) break;
     if (chunk % kCheck != 0) continue;
     __syncthreads();
     const int n = s_n;
@@ -246,7 +251,7 @@ beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slic
   if (lane == 0) s_top[warp] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kSelWarps; ++w) top = fmaxf(top, s_top[w]);
+  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_top[w]);
   if (top > -INFINITY) all *= double(ex2f((mine - top) * kLog2e));
 #pragma unroll
   for (int s = 16; s >= 1; s >>= 1) all += __shfl_xor_sync(0xffffffffu, all, s);
@@ -255,12 +260,12 @@ beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slic
   uint64_t* const out = best + part * num;
   if (room && n <= kList) {
     rank(n);
-    for (int i = tid; i < num; i += kSelThreads) out[i] = i < n ? s_best[i] : 0;
+    for (int i = tid; i < num; i += kThreads) out[i] = i < n ? s_best[i] : 0;
   } else {
     uint64_t last = ~uint64_t(0);
     for (int r = 0; r < num; ++r) {
       uint64_t key = 0;
-      for (int c = v0 + tid; c < v1; c += kSelThreads) {
+      for (int c = v0 + tid; c < v1; c += kThreads) {
         const uint64_t k = key_of(Elem<T>::to_f(p[c]), c);
         if (k < last) key = max64(key, k);
       }
@@ -270,14 +275,14 @@ beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slic
       if (lane == 0) s_key[warp] = key;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < kSelWarps; ++w) key = max64(key, s_key[w]);
+      for (int w = 0; w < kWarps; ++w) key = max64(key, s_key[w]);
       if (tid == 0) out[r] = key;
       last = key;
     }
   }
   if (tid == 0) {
     all = 0.;
-    for (int w = 0; w < kSelWarps; ++w) all += s_sum[w];
+    for (int w = 0; w < kWarps; ++w) all += s_sum[w];
     slices[part] = Slice{top, 0.f, all};
   }
 }
@@ -286,29 +291,31 @@ beam_slices_kernel(const T* __restrict__ logits, int64_t stride, int V, int slic
 // ranks at a time as the threads can take; once a whole rank holds nothing ahead of the num-th highest so far, no further one does.  What
 // the argument above on lanes and warps does not rule out goes side by side in shared memory, where each counts those ahead of it.
 // Bound by latency: two round trips to global memory, a logarithm in 64 bits, and three or four barriers for every set of ranks (one or two sets in
-// general).  16 groups of 16 beams of 128256, 32 of them: the join is 12 us of 55 (the slices' kernel 43), where it was 61 with all 1024 candidates
+// general).  16 groups of 16 beams of 128256, 32 of them: 38 us for both kernels, where the join alone took 61 with all 1024 candidates
 // of a group in any order.
-__global__ void __launch_bounds__(kSelThreads)
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads)
 beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ best, const float* __restrict__ scores,
                  const uint8_t* __restrict__ finished, const void* __restrict__ logits, int64_t stride, int dtype, int beams, int n_slices, int V,
                  int num, int end_token, float* __restrict__ out_scores, int64_t* __restrict__ out_tokens, int64_t* __restrict__ out_parents) {
+  constexpr int kWarps = kThreads / 32;
   __shared__ double s_total[kMostBeams];                   // logsumexp of a beam's logits less their maximum (which may be far beyond it)
   __shared__ float s_score[kMostBeams], s_top[kMostBeams];
   __shared__ uint8_t s_kind[kMostBeams];
-  __shared__ double s_sum[kSelWarps];
+  __shared__ double s_sum[kWarps];
   // an item: the value's order in 64 bits, and beam << 32 | token
-  __shared__ uint64_t s_order[kSelThreads + kMostNum], s_place[kSelThreads + kMostNum], s_best[2][kMostNum];
-  __shared__ uint32_t s_least[2][kSelWarps], s_close[kMostBeams / 32];       // beams that are too close to one another
+  __shared__ uint64_t s_order[kThreads + kMostNum], s_place[kThreads + kMostNum], s_best[2][kMostNum];
+  __shared__ uint32_t s_least[2][kWarps], s_close[kMostBeams / 32];       // beams that are too close to one another
   __shared__ int s_n;
   enum { kOpen, kFinished, kDead };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t g = blockIdx.x;
   // Lists of the group, and how a set of candidates is made of them: whole ranks of all lists, or a part of one.
-  const int lists = beams * n_slices, ranks = lists <= kSelThreads ? kSelThreads / lists : 1, parts = (lists + kSelThreads - 1) / kSelThreads;
+  const int lists = beams * n_slices, ranks = lists <= kThreads ? kThreads / lists : 1, parts = (lists + kThreads - 1) / kThreads;
   const int sets = parts > 1 ? num * parts : (num + ranks - 1) / ranks;
   // (a list's ranks side by side, so that every warp has some of the first ones)
   const int my_list = tid / ranks, my_rank = tid % ranks;
-  auto list_of = [&](int set) { return parts > 1 ? set % parts * kSelThreads + tid : my_list; };
+  auto list_of = [&](int set) { return parts > 1 ? set % parts * kThreads + tid : my_list; };
   auto rank_of = [&](int set) { return parts > 1 ? set / parts : set * ranks + my_rank; };
   const uint64_t* const mine = best + g * lists * num;
   auto fetch = [&](int set) -> uint64_t {
@@ -317,7 +324,7 @@ beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ 
   };
   cudaGridDependencySynchronize();
   const uint64_t first_key = fetch(0);
-  for (int k = warp; k < beams; k += kSelWarps) {          // a warp a beam
+  for (int k = warp; k < beams; k += kWarps) {          // a warp a beam
     const int64_t row = g * beams + k;
     const Slice* const part = slices + row * n_slices;
     Slice one{-INFINITY, 0.f, 0.};
@@ -378,11 +385,11 @@ beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ 
       const uint32_t high = uint32_t(order >> 32);
       const uint32_t sorted = sorted_in_warp(high, lane);
       if (lane == (num <= 32 ? num : 32) - 1) s_least[0][warp] = num <= 32 ? sorted : 0;
-      if (lane == (num + kSelWarps - 1) / kSelWarps - 1) s_least[1][warp] = sorted;
+      if (lane == (num + kWarps - 1) / kWarps - 1) s_least[1][warp] = sorted;
       __syncthreads();
       uint32_t most = 0, all = ~0u;
 #pragma unroll
-      for (int w = 0; w < kSelWarps; ++w) {
+      for (int w = 0; w < kWarps; ++w) {
         most = max(most, s_least[0][w]);
         all = min(all, s_least[1][w]);
       }
@@ -401,7 +408,7 @@ beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ 
       fresh = (parts > 1 && set % parts != 0 && fresh) || n > kept || !least_order;
       if (n > kept) {
         // the lanes of a group of 8 count their eighths of what is ahead of a candidate (one thread a candidate: 62 candidates take 4 us)
-        for (int first = 0; first < n; first += kSelThreads / 8) {
+        for (int first = 0; first < n; first += kThreads / 8) {
           const int i = first + tid / 8;
           const uint64_t o = i < n ? s_order[i] : 0, q = i < n ? s_place[i] : 0;
           int ahead = 0;
@@ -462,7 +469,7 @@ beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ 
       const int64_t from = (g * beams + k) * stride;
       const double top = s_top[k];
       double sum = 0.;
-      for (int v = tid; v < V; v += kSelThreads) {
+      for (int v = tid; v < V; v += kThreads) {
         const float x = dtype == MB200_F32 ? static_cast<const float*>(logits)[from + v]
                                            : __bfloat162float(static_cast<const __nv_bfloat16*>(logits)[from + v]);
         sum += exp(double(x) - top);
@@ -474,7 +481,7 @@ beam_join_kernel(const Slice* __restrict__ slices, const uint64_t* __restrict__ 
       __syncthreads();
       if (tid == 0) {
         sum = 0.;
-        for (int w = 0; w < kSelWarps; ++w) sum += s_sum[w];
+        for (int w = 0; w < kWarps; ++w) sum += s_sum[w];
         s_total[k] = log(sum);
       }
     }
@@ -617,17 +624,26 @@ beam_reorder_kernel(const int64_t* __restrict__ slots, const int64_t* __restrict
 
 using namespace mb200;
 
-// Logits of a CTA: whole chunks, as many as leave about four CTAs for every SM.
-static int64_t slice_of(int64_t rows, int64_t V) {
-  const int64_t chunks = (V + kSelChunk - 1) / kSelChunk, wanted = int64_t(sm_count()) * 4 / (rows > 0 ? rows : 1);
-  const int64_t slices = wanted < 1 ? 1 : min64(wanted, chunks);
-  return (chunks + slices - 1) / slices * kSelChunk;
-}
+// Logits of a CTA: whole chunks, as many as leave about four CTAs (of 256 threads, two of 512) for every SM.
+struct SelectPlan {
+  int threads, join_threads;
+  int64_t slice, n_slices;
+  SelectPlan(int64_t rows, int64_t beams, int64_t V, int num) {
+    auto chunks = [&](int t) { return (V + t * kSelPer - 1) / (t * kSelPer); };
+    // Where CTAs of 256 threads take several chunks, 512 find a better threshold in their first one (us with 256 / 512: 64 x 4 x 50280, 4 of
+    // them 17.9 / 18.0; 16 x 16 x 128256, 32 of them 55 / 43); where not, they halve the CTAs (5 x 32001 9.0 / 10.4).
+    threads = rows * chunks(256) > int64_t(sm_count()) * 4 ? 512 : 256;
+    const int64_t all = chunks(threads), wanted = int64_t(sm_count()) * (1024 / threads) / (rows > 0 ? rows : 1), slices = wanted < 1 ? 1 : min64(wanted, all);
+    slice = (all + slices - 1) / slices * threads * kSelPer;
+    n_slices = (V + slice - 1) / slice;
+    // A thread a candidate at a time: 8 x 4 of them 18.0 us with 256, 19.1 with 512; 40 x 10 9.8 and 9.0, 32 x 32 43 and 38.
+    join_threads = beams * n_slices * num > 256 ? 512 : 256;
+  }
+};
 
 extern "C" int64_t mb200_beam_select_scratch_bytes(int64_t groups, int64_t beams, int64_t V, int num) {
   if (groups < 1 || beams < 1 || V < 1 || num < 1) return 0;
-  const int64_t slice = slice_of(groups * beams, V);
-  return groups * beams * ((V + slice - 1) / slice) * int64_t(sizeof(Slice) + num * sizeof(uint64_t));
+  return groups * beams * SelectPlan(groups * beams, beams, V, num).n_slices * int64_t(sizeof(Slice) + num * sizeof(uint64_t));
 }
 
 extern "C" int mb200_beam_select(const void* logits, const float* scores, const uint8_t* finished, void* scratch, float* out_scores,
@@ -641,13 +657,17 @@ extern "C" int mb200_beam_select(const void* logits, const float* scores, const 
   if (!logits || !scores || !scratch || !out_scores || !out_tokens || !out_parents) return MB200_EINVAL;
   if (!aligned16(scratch)) return MB200_EALIGN;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t rows = groups * beams, slice = slice_of(rows, V), n_slices = (V + slice - 1) / slice;
+  const int64_t rows = groups * beams;
+  const SelectPlan plan(rows, beams, V, num);
+  const int64_t slice = plan.slice, n_slices = plan.n_slices;
   if (beams * n_slices * num >= (int64_t(1) << 31)) return MB200_ETOOBIG;
   Slice* slices = static_cast<Slice*>(scratch);
   uint64_t* best = reinterpret_cast<uint64_t*>(slices + rows * n_slices);
   const dim3 grid(static_cast<unsigned>(n_slices), static_cast<unsigned>(rows));
   const bool vec = aligned16(logits) && row_stride * (dtype == MB200_F32 ? 4 : 2) % 16 == 0;
-#define MB200_SLICES(TT, VEC) beam_slices_kernel<TT, VEC><<<grid, kSelThreads, 0, st>>>((const TT*)logits, row_stride, int(V), int(slice), num, slices, best)
+#define MB200_SLICES(TT, VEC)                                                                                                                   \
+  (plan.threads == 512 ? beam_slices_kernel<TT, VEC, 512> : beam_slices_kernel<TT, VEC, 256>)<<<grid, unsigned(plan.threads), 0, st>>>(         \
+      (const TT*)logits, row_stride, int(V), int(slice), num, slices, best)
   if (dtype == MB200_F32) { if (vec) MB200_SLICES(float, true); else MB200_SLICES(float, false); }
   else { if (vec) MB200_SLICES(__nv_bfloat16, true); else MB200_SLICES(__nv_bfloat16, false); }
 #undef MB200_SLICES
@@ -657,10 +677,10 @@ extern "C" int mb200_beam_select(const void* logits, const float* scores, const 
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t how{};
-  how.gridDim = dim3(unsigned(groups)); how.blockDim = dim3(kSelThreads); how.stream = st; how.attrs = &early; how.numAttrs = 1;
+  how.gridDim = dim3(unsigned(groups)); how.blockDim = dim3(unsigned(plan.join_threads)); how.stream = st; how.attrs = &early; how.numAttrs = 1;
   const Slice* slices_c = slices;
   const uint64_t* best_c = best;
-  if (cudaLaunchKernelEx(&how, beam_join_kernel, slices_c, best_c, scores, finished, logits, row_stride, dtype, int(beams), int(n_slices), int(V), num,
+  if (cudaLaunchKernelEx(&how, plan.join_threads == 512 ? beam_join_kernel<512> : beam_join_kernel<256>, slices_c, best_c, scores, finished, logits, row_stride, dtype, int(beams), int(n_slices), int(V), num,
                          int(end_token), out_scores, out_tokens, out_parents) != cudaSuccess)
     return MB200_ELAUNCH;
   return check_launch();
