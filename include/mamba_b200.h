@@ -498,8 +498,9 @@ int mb200_conv_step_slots(const void* xin, void* windows, const int64_t* slots, 
  * lowest k V + v.  logits: groups * beams rows of V, row_stride apart; scores (groups, beams).  finished (groups, beams), or NULL: a finished
  * beam has one continuation, end_token, at its own score.  A beam whose score is not finite, or whose logits hold a NaN or +inf or nothing above
  * -inf, has none.  Where a group has fewer than num, the rest are the lowest k V + v left, at -inf.
- * Out: out_scores, out_tokens (v), out_parents (k), each (groups, num).  At most 64 beams, num at most 64 (MB200_ETOOBIG);
- * scratch: mb200_beam_select_scratch_bytes bytes, 16-byte aligned, for one call at a time. */
+ * Out: out_scores, out_tokens (v), out_parents (k), each (groups, num).  At most 64 beams a group and 65535 in all, num at
+ * most 64, V below 2^30 (MB200_ETOOBIG).  scratch: mb200_beam_select_scratch_bytes bytes (asked for with the same device current: it depends on
+ * the number of SMs), 16-byte aligned, for one call at a time. */
 int64_t mb200_beam_select_scratch_bytes(int64_t groups, int64_t beams, int64_t V, int num);
 int mb200_beam_select(const void* logits, const float* scores, const uint8_t* finished, void* scratch, float* out_scores,
                       int64_t* out_tokens, int64_t* out_parents, int64_t groups, int64_t beams, int64_t V, int num, int64_t end_token,

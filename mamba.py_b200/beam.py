@@ -16,7 +16,7 @@ def beam_select(logits, scores, num=None, finished=None, end_token=None):
     token's log-softmax; equal ones come in the order of parent and token.  `num` is K by default; 2 K lets a caller put ended ones aside.
     A beam that `finished` (G, K) bool marks has one continuation, `end_token`, at its own score.  A beam whose score is not finite (the
     others of a search's first step: -inf) or whose logits hold a NaN, +inf or nothing above -inf has none.  Places left are filled with
-    the lowest tokens of the lowest beams at -inf.  K and num are at most 64."""
+    the lowest tokens of the lowest beams at -inf.  K and num are at most 64, G * K at most 65535."""
     return _host().beam_select(logits, scores, num, finished, end_token)
 
 
