@@ -649,10 +649,11 @@ extern "C" int64_t mb200_beam_select_scratch_bytes(int64_t groups, int64_t beams
 extern "C" int mb200_beam_select(const void* logits, const float* scores, const uint8_t* finished, void* scratch, float* out_scores,
                                  int64_t* out_tokens, int64_t* out_parents, int64_t groups, int64_t beams, int64_t V, int num, int64_t end_token,
                                  int64_t row_stride, int dtype, void* stream) {
-  if (groups < 0 || beams < 1 || V < 1 || num < 1 || num > beams * V) return MB200_EINVAL;
+  if (groups < 0 || beams < 1 || V < 1 || num < 1) return MB200_EINVAL;
   if (dtype != MB200_F32 && dtype != MB200_BF16) return MB200_EDTYPE;
   if (finished && (end_token < 0 || end_token >= V)) return MB200_EINVAL;
-  if (beams > kMostBeams || num > kMostNum || V >= (int64_t(1) << 30) || groups * beams > 65535) return MB200_ETOOBIG;
+  if (beams > kMostBeams || num > kMostNum || V >= (int64_t(1) << 30) || groups > 65535 || groups * beams > 65535) return MB200_ETOOBIG;
+  if (num > beams * V) return MB200_EINVAL;
   if (groups == 0) return MB200_OK;
   if (!logits || !scores || !scratch || !out_scores || !out_tokens || !out_parents) return MB200_EINVAL;
   if (!aligned16(scratch)) return MB200_EALIGN;

@@ -893,7 +893,9 @@ extern "C" int mb200_sscan_packed_fwd(const mb200_packed* seqs, const void* x, c
                                       float* pieces, int64_t ED, int N, int64_t x_sl, int64_t d_sl, int64_t z_sl, int64_t b_sl,
                                       int64_t c_sl, int64_t y_sl, int64_t piece_len, int64_t parts, int dtype, int flags, void* stream) {
   if (const int rc = packed_check(seqs)) return rc;
-  if (ED < 0 || piece_len < 0 || parts < 1 || piece_len % (parts * kTile)) return MB200_EINVAL;
+  if (ED < 0 || piece_len < 0 || parts < 1) return MB200_EINVAL;
+  if (piece_len >= (int64_t(1) << 30) || parts >= (int64_t(1) << 20)) return MB200_ETOOBIG;
+  if (piece_len % (parts * kTile)) return MB200_EINVAL;
   if (dtype != MB200_F32 && dtype != MB200_BF16) return MB200_EDTYPE;
   if (N != 8 && N != 16 && N != 32 && N != 64) return MB200_ENSTATE;
   if (seqs->rows == 0 || ED == 0) return MB200_OK;

@@ -47,6 +47,7 @@ def test_scan_arguments():
 
     for f, n in ((fwd, 12), (bwd, 20)):
         assert f(ED=-1) == EINVAL and f(piece=-16) == EINVAL and f(piece=24) == EINVAL and f(piece=48, parts=2) == EINVAL and f(parts=0) == EINVAL
+        assert f(piece=1 << 40) == ETOOBIG and f(parts=1 << 60) == ETOOBIG and f(piece=16, parts=1 << 60) == ETOOBIG
         assert f(dtype=2) == EDTYPE and f(N=12) == ENSTATE
         assert f(s=_seqs(rows=0)) == 0 and f(ED=0) == 0                  # nothing to do
         assert f(ptrs=[None] + [P] * (n - 1)) == EINVAL                  # x
@@ -98,6 +99,7 @@ def test_beam_arguments():
     assert select(groups=-1) == EINVAL and select(beams=0) == EINVAL and select(V=0) == EINVAL and select(num=0) == EINVAL and select(num=28) == EINVAL
     assert select(dtype=2) == EDTYPE and select(finished=P, end=9) == EINVAL and select(finished=P, end=-1) == EINVAL
     assert select(beams=65) == ETOOBIG and select(V=99, num=65) == ETOOBIG and select(V=1 << 30) == ETOOBIG and select(groups=65536) == ETOOBIG
+    assert select(groups=1 << 60, beams=64) == ETOOBIG and select(V=1 << 62) == ETOOBIG
     assert select(logits=None) == EINVAL and select(scratch=None) == EINVAL and select(scratch=P + 8) == -4 and select(groups=0) == 0
     assert lib.mb200_beam_select_scratch_bytes(0, 3, 9, 3) == 0 and lib.mb200_beam_select_scratch_bytes(1, 1, 0, 1) == 0
 
