@@ -15,16 +15,6 @@ namespace {
 constexpr int kPkThreads = 256, kPkWarps = kPkThreads / 32, kPkResident = 3;
 constexpr int kPkChunk = 32, kPkGroup = 8;              // rows of a warp; rows whose loads go out together
 
-// Both sigmoids of a pair from one reciprocal: 1 / (a b) times the other.  The exponentials stay below 2^60 for that (a sigmoid of less is 2^-60).
-// The special function unit, which takes 16 cycles for two results of a warp and was busy for 19 of 42 us at 8000 x 5120, has a quarter less to do.
-__device__ __forceinline__ Pk<1> psigmoid_pk(Pk<1> a) { return psigmoid(a); }
-__device__ __forceinline__ Pk<2> psigmoid_pk(Pk<2> a) {
-  const float2 m = __fmul2_rn(a.v, make_float2(-kLog2e, -kLog2e));
-  const float2 d = __fadd2_rn(make_float2(ex2f(fminf(m.x, 60.f)), ex2f(fminf(m.y, 60.f))), make_float2(1.f, 1.f));
-  const float r = rcpf(d.x * d.y);
-  return {__fmul2_rn(make_float2(r, r), make_float2(d.y, d.x))};
-}
-
 // Where sequences begin: a bit for every row from `base` on.
 struct Firsts {
   const unsigned* bits;
@@ -155,7 +145,7 @@ conv1d_silu_packed_fwd_kernel(const Packed seqs, const T* __restrict__ x, const 
         acc = pfma(wk[i][2], win[i][2], acc);
         acc = pfma(wk[i][3], xn[i], acc);
         win[i][0] = win[i][1]; win[i][1] = win[i][2]; win[i][2] = xn[i];
-        o[i] = pmul(acc, psigmoid_pk(acc));
+        o[i] = pmul(acc, psigmoid(acc));
       }
       return pack<T, V, W>(o);
     };
@@ -246,6 +236,8 @@ conv1d_silu_packed_fwd_kernel(const Packed seqs, const T* __restrict__ x, const 
 // each, a lane 8 bytes of channels, and store y.  A CTA walks through every gridDim.y-th box of its channels.
 // bfloat16, us so / one channel a thread / four: 8000 x 5120, 12 sequences 32.9 / - / 42.2 (a copy 27.4), 16000 x 1536 20.2 / 30.1 / 26.5, 4000 x 1536
 // 8.8 / 10.3 / 12.2, 2999 x 1000 7.4 / 6.9 / 9.4, 1000 x 512 4.2 / 5.0 / 9.1.
+// Each sigmoid has a reciprocal of its own.  One for the product of a pair's sums saves nothing (8192 x 5120 30.4 and 30.4, the backward at 16000 x 1536
+// 38.1 for 39.4), runs out of range far below zero and leaves a sigmoid near 1 a rounding off, which the derivative multiplies with the preactivation.
 constexpr int kTcRows = 32, kTcBox = kConvK - 1 + kTcRows + kConvK - 2, kTcBytes = 256, kTcStages = 4, kTcWarps = 4, kTcResident = 5;
 constexpr int kTcThreads = 32 * (kTcWarps + 1);
 
@@ -351,7 +343,7 @@ conv1d_silu_packed_tma_kernel(const __grid_constant__ CUtensorMap map, const Pac
         acc = pfma(wk[i][2], win[i][2], acc);
         acc = pfma(wk[i][3], xn[i], acc);
         win[i][0] = win[i][1]; win[i][1] = win[i][2]; win[i][2] = xn[i];
-        o[i] = pmul(acc, psigmoid_pk(acc));
+        o[i] = pmul(acc, psigmoid(acc));
       }
       return pack<T, V, W>(o);
     };
@@ -529,7 +521,7 @@ conv1d_silu_packed_bwd_kernel(const Packed seqs, const T* __restrict__ x, const 
           F pre = bv[i];
 #pragma unroll
           for (int k = 0; k < kConvK; ++k) pre = pfma(wk[i][k], xw[i][(j + 1 + k) % kG], pre);
-          const F sg = psigmoid_pk(pre);
+          const F sg = psigmoid(pre);
           const F dp = pmul(pmul(g[i], sg), pfma(pre, pfma(sg, mone, one), one));
           dw_[i][j] = dp;
           // dx[t-3] = w3*dpre[t-3] + w2*dpre[t-2] + w1*dpre[t-1] + w0*dpre[t]
