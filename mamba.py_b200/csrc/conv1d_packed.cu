@@ -475,7 +475,7 @@ conv1d_silu_packed_bwd_kernel(const Packed seqs, const T* __restrict__ x, const 
       }
     }
     const F one = F::splat(1.f), mone = F::splat(-1.f), zero = F::splat(0.f);
-    const int own = t1 - t0, end = min(tail, t1 + kH) - t0;
+    const int own = max(0, min(t1, tail) - t0), end = min(tail, t1 + kH) - t0;
     CVec<T, V>* const mine = reinterpret_cast<CVec<T, V>*>(ring) + warp * (kStages * 2 * kG * 32) + lane;
     int stage = 0;
     auto ahead = [&](int s0, int to) {
@@ -555,6 +555,10 @@ conv1d_silu_packed_bwd_kernel(const Packed seqs, const T* __restrict__ x, const 
       else group(std::false_type{}, s0, f);
       if (kRing && ++stage == kStages) stage = 0;
     }
+    CVec<T, V> none;                                      // rows of no sequence, whatever the filter holds
+#pragma unroll
+    for (int i = 0; i < V; ++i) none.v[i] = Elem<T>::from_f(0.f);
+    for (int t = max(t0, tail); t < t1; ++t) cstore<T, V>(dx + int64_t(t) * dx_sl + e, none);
 #pragma unroll
     for (int i = 0; i < P; ++i) {
 #pragma unroll

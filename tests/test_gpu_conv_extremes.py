@@ -97,3 +97,17 @@ def test_infinities_and_nan(T, W, dtype, dense):
     s = torch.sigmoid(pre)
     slope = torch.cat([dy.double() * s * (1 + pre * (1 - s)), torch.zeros(3, W, dtype=torch.float64, device=DEV)])
     within(dx, sum(slope[3 - k:3 - k + T] * w.double()[:, 0, k] for k in range(4)), torch.nan_to_num(x, 0, 0, 0), dtype, 2)
+
+
+@pytest.mark.parametrize("T,W,dtype", SIZES)
+def test_rows_behind_the_last_sequence(T, W, dtype):
+    """Zeros, whatever the filter holds."""
+    import mamba_b200
+    x, w, b, dy = makes(T, W, dtype, [-5.0, 0.5, 3.0], T)
+    w[:, 0, 0], w[::2, 0, 3], b[1::3] = math.inf, math.nan, -math.inf
+    for lengths in ([T // 2], [T - 1], [7, 2, T - 12], []):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        y = mamba_b200.causal_conv1d_silu_packed(*leaves, cu_seqlens=cu_of(lengths))
+        dx, dw, db = torch.autograd.grad(y, leaves, dy)
+        assert (y[sum(lengths):] == 0).all() and (dx[sum(lengths):] == 0).all(), lengths
+    assert (dw == 0).all() and (db == 0).all()              # (of no sequence at all)
