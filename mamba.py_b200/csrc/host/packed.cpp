@@ -345,6 +345,7 @@ Tensor conv1d_silu_packed(const Tensor& x, const Tensor& weight, const OptTensor
   const auto dt = act_dtype(x);
   const bool grad = wants_grad(x, weight, bias);
   const int64_t T = x.size(0), W = x.size(1), K = weight.size(-1);
+  TORCH_CHECK(K == 4, "mamba_b200: the convolution of packed sequences takes filters of 4 taps (d_conv 4), got ", K);
   if (windows.defined()) {
     check_pool(windows, {W, K - 1}, dt, "windows");
     TORCH_CHECK(!grad, "mamba_b200: a convolution that leaves its windows in slots has no gradient; call it under torch.no_grad()");

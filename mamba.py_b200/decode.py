@@ -13,7 +13,8 @@ from .beam import beam_reorder, beam_select
 
 class StatePool:
     """The states and convolution windows of `slots` requests for every layer of a stack (an object with `layers` whose mixers have the
-    attributes of the reference's MambaBlock).  `dtype` is the activations': the windows have it, states are float32."""
+    attributes of the reference's MambaBlock).  `dtype` is the activations': the windows have it, states are float32.  Tokens and beams go
+    with any d_conv up to 8, prompts with 4 alone."""
 
     def __init__(self, stack, slots, dtype=torch.float32, device="cuda"):
         self.stack = stack
