@@ -44,9 +44,10 @@ class StatePool:
 
 @torch.no_grad()
 def beam_search(pool, embed, head, logits, slots, steps, end_token=None):
-    """`steps` tokens of a beam search.  slots (G, K): a group's prompt has been read into slots[:, 0], and `logits` (G, V) are those of its
-    last token; embed(tokens (B,)) -> (B, D) and head(x (B, D)) -> (B, V) are the model's ends.  Returns (tokens (G, K, steps), scores
-    (G, K)), best beam first; a beam that has chosen `end_token` goes on choosing it."""
+    """`steps` tokens of a beam search.  slots (G, K), all different: slots[:, 0] has read a group's prompt (and whatever tokens have come
+    since), the others may hold anything; `logits` (G, V) are those of the last token that slots[:, 0] has read.  embed(tokens (B,)) -> (B, D)
+    and head(x (B, D)) -> (B, V) are the model's ends.  Returns (tokens (G, K, steps), scores (G, K)), best beam first; a beam that has chosen
+    `end_token` goes on choosing it."""
     G, K = slots.shape
     scores = torch.full((G, K), float("-inf"), device=slots.device)
     scores[:, 0] = 0.0
