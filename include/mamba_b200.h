@@ -441,8 +441,8 @@ int mb200_block_step(const mb200_block_step_args* args, float* scratch, void* ba
  * the device, read by the kernels alone, so that a captured graph can be replayed with other lengths; whatever they hold, nothing outside
  * the tensors is touched.
  * slots (sequences), or NULL: where in a pool of n_slots entries the sequence's state lies; one outside 0 .. n_slots - 1 means that it
- * has none: it starts from zero and leaves nothing.  A slot that is given twice is left holding either sequence's state.  resume (sequences),
- * or NULL for none: whether a sequence starts from what its slot holds.  A sequence without rows leaves its slot as it is. */
+ * has none: it starts from zero and leaves nothing.  The others must differ: what a slot that is given twice holds afterwards, and what its sequences
+ * give if they resume, is any mixture of theirs.  resume (sequences), or NULL for none: whether a sequence starts from what its slot holds.  A sequence without rows leaves its slot as it is. */
 typedef struct {
   const int32_t* cu_seqlens;
   int64_t sequences, rows;      /* at most 65534, and below 2^30 */
@@ -484,7 +484,7 @@ int mb200_conv1d_silu_packed_bwd(const mb200_packed* seqs, const void* x, const 
 
 /* mb200_ssm_step_params and mb200_conv_step on pools: row b's state is entry slots[b] of states (n_slots, ED, N), its window entry slots[b] of
  * windows (n_slots, ED, K-1), both updated in place.  A row with a slot outside 0 .. n_slots - 1 gives zeros and updates nothing (padding of
- * a captured batch).  A slot that is given twice is left holding either row's state. */
+ * a captured batch).  The others must differ: what a slot that is given twice holds afterwards, and its rows' outputs, are any mixture of theirs. */
 int mb200_ssm_step_slots(const void* x, const void* delta, const void* z, const void* A, int A_dtype, int A_is_log,
                          const void* Bm, const void* Cm, const void* D, int D_dtype, const void* delta_bias, int bias_dtype,
                          float* states, const int64_t* slots, int64_t n_slots, void* y, int64_t B, int64_t ED, int N,
