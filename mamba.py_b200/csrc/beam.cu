@@ -68,9 +68,11 @@ __device__ __forceinline__ uint32_t sorted_in_warp(uint32_t x, int lane) {
 // highest, is K.  Whatever reaches K, in the chunks that follow too (about num a chunk, if they are alike), is put side by side with its place, and
 // every item counts those ahead of it; between chunks the num-th of them becomes the new K.  That may be a
 // value that very many logits share (a mask's): equal to K, then, counts only up to the num-th place that does, of which there are num in the
-// first chunk or none.  Should a chunk have more than there is room for all the same (ascending logits may), num rounds over the slice find the highest.
-// Bound: 6 instructions a logit (load and conversion, maximum, half of a difference, product and sum, ex2), which is near the time that its 2 bytes take
-// from HBM, and some 2 us a CTA for the first chunk's sort and the counts at the end.  So a CTA takes as many chunks as leave
+// first chunk or none.  Should a chunk have more than there is room for all the same (ascending logits may, and a first chunk that a mask empties makes
+// the next one), num rounds over the slice find the highest.
+// Bound: 6 instructions a logit that it cannot do without (load and conversion, maximum, half of a difference, product and sum, ex2) would take about as
+// long as its 2 bytes from HBM.  It executes 18 (288 a warp for 512 logits: bounds, thresholds, sort and counts are the others) at half the issue slots and
+// takes 4 times as long as the bytes, some 2 us of a CTA's time for the first chunk's sort and the counts at the end.  So a CTA takes as many chunks as leave
 // 1024 threads for every SM, with the next chunk's loads in flight.  64 x 4 x 50280 in bfloat16: 58 us with a CTA to every 8192 logits and a count of
 // all threads' highest, 25 with the warps' sort, 22 with several chunks a CTA, 18 with the join's work and the exponentials' in pairs.
 template <typename T, bool kVec, int kThreads>

@@ -401,7 +401,7 @@ conv1d_silu_packed_tma_kernel(const __grid_constant__ CUtensorMap map, const Pac
 // As on rectangles the windows hold as many rows as a group, dx trails by three rows, and the 4 warps of a CTA add their sums in shared memory.
 // Of large tensors a thread takes 8 bytes of channels, and rows come through a ring in shared memory, groups ahead of the arithmetic: each thread copies
 // what it reads itself, so its own waits are all it takes, and no register holds what is on its way.  16000 x 1536 without / with the ring: float32
-// 70 (four channels) / 52 us (two; four 57), bfloat16 51 / 40 (two channels: 45).  Four stages of the ring take the L1 that the copies pass through
+// 70 (four channels) / 52 us (two; four 57), bfloat16 51 / 38 (two channels: 45).  Four stages of the ring take the L1 that the copies pass through
 // (float32 62), two cost bfloat16 2 us.  Then bfloat16 waits for issue slots (half of them, with 13 warps an SM), float32 for HBM (5.6 TB/s).
 constexpr int kPkBwdThreads = 128, kPkBwdWarps = kPkBwdThreads / 32, kPkBwdChunkMost = 128;
 constexpr int kPkBwdStages = 3;                          // groups of four rows of x and dy
@@ -599,10 +599,10 @@ int packed_chunk(int64_t rows, int64_t cols, int warps, int resident, int unit, 
   return best;
 }
 
-// Channels of a thread of the backward: 8 bytes of them save instructions, one gives more warps.  us so / with one, with the launches around it:
+// Channels of a thread of the backward: 8 bytes of them save instructions, one gives more warps.  us so / with one, kernels in a graph:
 //            1000 x 512   3000 x 1000   8000 x 512   4000 x 1536   2000 x 5120   8000 x 1536   16000 x 1536
-// float32     5.7 / 5.9    12.0 / 10.2    15.0 / 13.0  17.9 / 25.8   26.0 / 44.2   33.1 / 53.2   52.2 / 90.1
-// bfloat16    7.2 / 5.5    12.7 / 11.0    15.0 / 11.9  18.2 / 16.2   23.7 / 34.5   26.3 / 45.6   39.8 / 86.4
+// float32     5.2 / 4.7     9.9 / 9.2    11.4 / 11.8  16.0 / 21.5   24.6 / 40.9   29.7 / 49.3   53.5 / 90.5
+// bfloat16    6.3 / 4.8    11.6 / 10.3   13.9 / 11.4  16.6 / 15.9   22.1 / 35.3   24.8 / 43.7   38.0 / 84.7
 bool one_channel(int64_t values, int dtype) { return values <= (dtype == MB200_F32 ? int64_t(9) << 19 : int64_t(7) << 20); }
 
 int check_conv(const mb200_packed* seqs, int64_t ED, int K, int dtype) {

@@ -32,10 +32,10 @@ __device__ __forceinline__ int op_index(int t, int c, int te) {
   return t * te + swz(t, c >> 1) * 2 + (c & 1);
 }
 
-// Exponents delta * A log2(e) of decays in the packed kernels.  ex2.approx comes out low: by 0.5e-8 of its value on average for exponents above -0.004,
+// Exponents delta * A log2(e) of decays in the packed tensor-map kernels (the generic ones and the steps on slots go without).  ex2.approx comes out low: by 0.5e-8 of its value on average for exponents above -0.004,
 // 2.6e-8 from there to -0.03, 1.7e-8 to -0.12, 1.0e-8 to -0.5 (measured on 2^22 arguments each), and a recurrence that forgets slowly adds that up over
 // all the steps that it remembers.  A constant in the place of the product's zero costs nothing and takes 1.0e-8 off: the error of dA
-// against 64 bits on 2999 x 1000 in float32 goes from 1.3e-6 to 0.8e-6 (one rounding each: 0.45e-6).
+// against 64 bits on 2999 x 1000 in float32 goes from 1.3e-6 to 0.8e-6 (one rounding each: 0.45e-6).  A step that does not decay stays one: ex2 of it is 1.
 template <bool kPacked>
 __device__ __forceinline__ float2 decay_exponent(float2 delta, float2 A2) {
   if constexpr (kPacked) return __ffma2_rn(delta, A2, make_float2(1.44e-8f, 1.44e-8f));
