@@ -84,13 +84,13 @@ def stream():
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("W,N,dtype", [(32, 16, torch.float32), (40, 16, torch.bfloat16), (37, 16, torch.float32), (24, 8, torch.bfloat16), (20, 64, torch.float32)])
-@pytest.mark.parametrize("piece,parts", [(0, 1), (16, 1), (96, 2)])
+# (cut for d_state 16 and tensors that tensor maps describe)
+@pytest.mark.parametrize("W,N,dtype,piece,parts", [(32, 16, torch.float32, 0, 1), (32, 16, torch.float32, 16, 1), (32, 16, torch.float32, 96, 2),
+                                                   (40, 16, torch.bfloat16, 0, 1), (40, 16, torch.bfloat16, 16, 1), (40, 16, torch.bfloat16, 96, 2),
+                                                   (37, 16, torch.float32, 0, 1), (24, 8, torch.bfloat16, 0, 1), (20, 64, torch.float32, 0, 1)])
 def test_scan(kind, W, N, dtype, piece, parts):
     from mamba_b200 import _lib
     lib, T, S, code = _lib.load(), 300, 4, _lib.dtype_code(dtype)
-    if piece and (N != 16 or W == 37):
-        pytest.skip("cut for d_state 16 and tensors that tensor maps describe")
     f, t = Frames(), inputs(0, T, W, N, dtype)
     x, delta, z, dy = (f.rows(T, W, dtype=dtype, value=t[k]) for k in ("x", "delta", "z", "x"))
     B, C = (f.rows(T, N, dtype=dtype, value=t[k]) for k in ("B", "C"))
